@@ -429,6 +429,100 @@ RSC_API rsc_status rsc_shard_collect(const uint32_t *d_ready_results, uint32_t s
                                      uint32_t *d_out_ids, int32_t *d_out_status,
                                      float *d_out_probs, void *stream);
 
+/*
+ * Verification of drafted tokens (no counterpart in the reference, whose
+ * generation loop draws one token per forward pass,
+ * crates/rusticide-model/src/generate.rs:60-110). The target model has scored
+ * the tokens that a draft proposed for each sequence; the call accepts a
+ * prefix of them and draws one more token, so that the output is distributed
+ * as if the target had been sampled token by token.
+ *
+ * For sequence b with n = n_draft[b] tokens t_0 .. t_{n-1} (0 <= n <=
+ * max_drafts, values outside are clamped), target distributions p_0 .. p_n and
+ * draft distributions q_0 .. q_{n-1}:
+ *   - tests run in order: t_i is accepted iff u_i * q_i(t_i) < p_i(t_i). A
+ *     draft without a distribution has q_i(t_i) = 1; a token outside the
+ *     vocabulary has p = 0 and is refused;
+ *   - a = the first refused test, or n. One more token is drawn: from the
+ *     positive part of p_a - q_a where a was refused (from p_a without t_a
+ *     where the draft has no distribution; from p_a itself should nothing be
+ *     left), from p_n where all were accepted. It is the first index whose
+ *     running weight exceeds u * (sum of the weights), the last one of
+ *     positive weight should rounding find none.
+ * Every decision is that of exact arithmetic on the given binary32 values, to
+ * 1e-13 relative; results do not depend on the batch around a sequence.
+ *
+ * d_out_tokens[b] (max_drafts + 1 uint32): the accepted tokens, the drawn one,
+ * then 0xffffffff. d_out_accepted[b] = a. d_out_status[b] is RSC_ROW_OK, or
+ * RSC_ROW_NO_VALID_TOKENS when a needed row has no distribution (no logit
+ * above -inf, or one of +inf): the accepted tokens hold, none is drawn. Rows
+ * and tokens behind position n are not read.
+ *
+ * Draws: d_uniforms (n_seqs x (max_drafts + 1) f32 in [0, 1)) holds u_i at
+ * column i and the last draw's u at column max_drafts; or d_rng_states (one
+ * state per sequence, rsc_rng_seed) gives them in order and advances by the
+ * draws that were consumed. Neither is read by a greedy call.
+ */
+typedef struct rsc_draft_batch {
+    size_t n_seqs;
+    size_t max_drafts;
+    size_t vocab;
+    const float *d_target;        /* target row i of sequence b (0 <= i <= n) at                */
+    size_t target_seq_stride;     /*   d_target + b * target_seq_stride + i * target_row_stride  */
+    size_t target_row_stride;
+    const float *d_draft;         /* draft rows (0 <= i < n), likewise; NULL: no distribution   */
+    size_t draft_seq_stride;
+    size_t draft_row_stride;
+    const uint32_t *d_draft_tokens; /* n_seqs x max_drafts                                     */
+    const int32_t *d_n_draft;     /* n_seqs; NULL: max_drafts each                              */
+} rsc_draft_batch;
+
+/*
+ * rsc_verify: the distributions are the softmax of the scaled logits (x *
+ * (1/T), NaN read as -inf) over the whole vocabulary, so params must have
+ * top-k off (0 or >= vocab) and top_p >= 1 (RSC_ERR_INVALID_ARGUMENT
+ * otherwise: such a distribution is verified from its records, below) and a
+ * finite 1/T > 0. Parameters of the argmax branch (T == 0 or top_k == 1)
+ * verify greedily: t_i is accepted iff it is the token rsc_greedy gives for
+ * the row, the last token is that of row a, and the draft rows are not read.
+ *
+ * d_workspace: rsc_verify_workspace_bytes(n_seqs, max_drafts, vocab) bytes, 16-byte
+ * aligned, not initialised, free again when the call's work on the stream is
+ * done. The handle gives the device; its capacity (max_rows, max_vocab) does not
+ * limit this call, and it lends no memory to it. Limits: vocab < 2^31, n_seqs *
+ * (2 * max_drafts + 1) <= 2^27 (RSC_ERR_CAPACITY).
+ */
+RSC_API size_t rsc_verify_workspace_bytes(size_t n_seqs, size_t max_drafts, size_t vocab);
+RSC_API rsc_status rsc_verify(rsc_sampler *sampler, const rsc_draft_batch *batch,
+                              const rsc_params *params, const float *d_uniforms,
+                              uint64_t *d_rng_states, void *d_workspace, size_t workspace_bytes,
+                              uint32_t *d_out_tokens, uint32_t *d_out_accepted,
+                              int32_t *d_out_status, void *stream);
+
+/*
+ * rsc_verify_survivors: the distributions are survivor records as rsc_sample_ex
+ * writes them (n, then ids ascending and their probabilities, cap slots a
+ * row): those of the target's n_seqs x (max_drafts + 1) rows and, unless
+ * `draft` is NULL, of the draft's n_seqs x max_drafts rows. The logits, strides
+ * and vocab of the batch are not read. A row whose d_status (nullable) is not
+ * RSC_ROW_OK passes that code on to its sequence when it is needed; one with n
+ * above cap reports RSC_ROW_INTERNAL, an empty one RSC_ROW_NO_VALID_TOKENS.
+ */
+typedef struct rsc_survivor_records {
+    const uint32_t *d_n;      /* rows: entries of each record */
+    const uint32_t *d_ids;    /* rows x cap                   */
+    const float *d_probs;     /* rows x cap                   */
+    const int32_t *d_status;  /* rows, nullable               */
+    size_t cap;
+} rsc_survivor_records;
+
+RSC_API rsc_status rsc_verify_survivors(rsc_sampler *sampler, const rsc_draft_batch *batch,
+                                        const rsc_survivor_records *target,
+                                        const rsc_survivor_records *draft, const float *d_uniforms,
+                                        uint64_t *d_rng_states, uint32_t *d_out_tokens,
+                                        uint32_t *d_out_accepted, int32_t *d_out_status,
+                                        void *stream);
+
 /* Number of kernel launches the library issued since the handle was created
  * (for the benchmark's launch count). */
 RSC_API uint64_t rsc_launch_count(const rsc_sampler *sampler);

@@ -55,6 +55,34 @@ pub(crate) struct RscSampleExtras {
     pub(crate) d_survivor_logprobs: *mut f32,
 }
 
+/// `rsc_draft_batch`: drafted tokens and the logits they are verified against.
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub(crate) struct RscDraftBatch {
+    pub(crate) n_seqs: usize,
+    pub(crate) max_drafts: usize,
+    pub(crate) vocab: usize,
+    pub(crate) d_target: *const f32,
+    pub(crate) target_seq_stride: usize,
+    pub(crate) target_row_stride: usize,
+    pub(crate) d_draft: *const f32,
+    pub(crate) draft_seq_stride: usize,
+    pub(crate) draft_row_stride: usize,
+    pub(crate) d_draft_tokens: *const u32,
+    pub(crate) d_n_draft: *const i32,
+}
+
+/// `rsc_survivor_records`.
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub(crate) struct RscSurvivorRecords {
+    pub(crate) d_n: *const u32,
+    pub(crate) d_ids: *const u32,
+    pub(crate) d_probs: *const f32,
+    pub(crate) d_status: *const i32,
+    pub(crate) cap: usize,
+}
+
 /// Opaque `rsc_sampler`.
 #[repr(C)]
 pub(crate) struct RscSampler {
@@ -290,6 +318,36 @@ unsafe extern "C" {
         n_shards: usize,
         my_shard: usize,
         step: u32,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub(crate) fn rsc_verify_workspace_bytes(
+        n_seqs: usize,
+        max_drafts: usize,
+        vocab: usize,
+    ) -> usize;
+    pub(crate) fn rsc_verify(
+        sampler: *mut RscSampler,
+        batch: *const RscDraftBatch,
+        params: *const RscParams,
+        d_uniforms: *const f32,
+        d_rng_states: *mut u64,
+        d_workspace: *mut c_void,
+        workspace_bytes: usize,
+        d_out_tokens: *mut u32,
+        d_out_accepted: *mut u32,
+        d_out_status: *mut i32,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub(crate) fn rsc_verify_survivors(
+        sampler: *mut RscSampler,
+        batch: *const RscDraftBatch,
+        target: *const RscSurvivorRecords,
+        draft: *const RscSurvivorRecords,
+        d_uniforms: *const f32,
+        d_rng_states: *mut u64,
+        d_out_tokens: *mut u32,
+        d_out_accepted: *mut u32,
+        d_out_status: *mut i32,
         stream: *mut c_void,
     ) -> c_int;
     pub(crate) fn rsc_launch_count(sampler: *const RscSampler) -> u64;

@@ -75,6 +75,36 @@ class RscSampleExtras(ctypes.Structure):
     ]
 
 
+class RscDraftBatch(ctypes.Structure):
+    """rsc_draft_batch: drafted tokens of a batch and the logits they are verified against."""
+
+    _fields_ = [
+        ("n_seqs", ctypes.c_size_t),
+        ("max_drafts", ctypes.c_size_t),
+        ("vocab", ctypes.c_size_t),
+        ("d_target", ctypes.c_void_p),
+        ("target_seq_stride", ctypes.c_size_t),
+        ("target_row_stride", ctypes.c_size_t),
+        ("d_draft", ctypes.c_void_p),
+        ("draft_seq_stride", ctypes.c_size_t),
+        ("draft_row_stride", ctypes.c_size_t),
+        ("d_draft_tokens", ctypes.c_void_p),
+        ("d_n_draft", ctypes.c_void_p),
+    ]
+
+
+class RscSurvivorRecords(ctypes.Structure):
+    """rsc_survivor_records."""
+
+    _fields_ = [
+        ("d_n", ctypes.c_void_p),
+        ("d_ids", ctypes.c_void_p),
+        ("d_probs", ctypes.c_void_p),
+        ("d_status", ctypes.c_void_p),
+        ("cap", ctypes.c_size_t),
+    ]
+
+
 # Every symbol the header declares, with its ctypes signature.
 _P = ctypes.c_void_p
 _SZ = ctypes.c_size_t
@@ -110,6 +140,12 @@ SIGNATURES = {
     "rsc_lmhead_sample": (_ST, [_P, _P, _P, _SZ, _SZ, _SZ, ctypes.POINTER(RscParams), _P, _P, _P,
                                 _P, _P, _P]),
     "rsc_expf": (_ST, [_P, _P, _SZ, _P]),
+    "rsc_verify_workspace_bytes": (_SZ, [_SZ, _SZ, _SZ]),
+    "rsc_verify": (_ST, [_P, ctypes.POINTER(RscDraftBatch), ctypes.POINTER(RscParams), _P, _P, _P, _SZ,
+                         _P, _P, _P, _P]),
+    "rsc_verify_survivors": (_ST, [_P, ctypes.POINTER(RscDraftBatch),
+                                   ctypes.POINTER(RscSurvivorRecords),
+                                   ctypes.POINTER(RscSurvivorRecords), _P, _P, _P, _P, _P, _P]),
     "rsc_launch_count": (ctypes.c_uint64, [_P]),
     "rsc_debug_hold_scratch": (_ST, [_P, ctypes.c_int, _P]),
 }

@@ -747,6 +747,115 @@ rsc_status rsc_shard_publish(uint32_t *const *d_ready_ptrs, size_t n_shards, siz
                                                  static_cast<cudaStream_t>(stream)));
 }
 
+size_t rsc_verify_workspace_bytes(size_t n_seqs, size_t max_drafts, size_t vocab) {
+    return rsc::verify_workspace_bytes(n_seqs, max_drafts, vocab);
+}
+
+namespace {
+
+// The checks that both forms of verification share.
+rsc_status check_verify(const rsc_sampler *s, const rsc_draft_batch *x, const uint32_t *out_tokens,
+                        const uint32_t *out_accepted, const int32_t *out_status) {
+    if (!s || !s->alive) return RSC_ERR_NOT_INITIALIZED;
+    if (!x) return RSC_ERR_INVALID_ARGUMENT;
+    if (x->n_seqs > rsc::kVerifyMaxRows || x->max_drafts > rsc::kVerifyMaxRows ||
+        x->n_seqs * (2 * x->max_drafts + 1) > rsc::kVerifyMaxRows)
+        return RSC_ERR_CAPACITY;
+    if (x->n_seqs == 0) return RSC_OK;
+    if (!out_tokens || !out_accepted || !out_status) return RSC_ERR_INVALID_ARGUMENT;
+    if (x->max_drafts > 0 && !x->d_draft_tokens) return RSC_ERR_INVALID_ARGUMENT;
+    return RSC_OK;
+}
+
+rsc::VerifyCall verify_call(const rsc_draft_batch &x, const float *uniforms, uint64_t *rng_states,
+                            uint32_t *out_tokens, uint32_t *out_accepted, int32_t *out_status) {
+    rsc::VerifyCall c{};
+    c.n_seqs = static_cast<uint32_t>(x.n_seqs);
+    c.max_drafts = static_cast<uint32_t>(x.max_drafts);
+    c.draft_tokens = x.d_draft_tokens;
+    c.n_draft = x.d_n_draft;
+    c.uniforms = uniforms;
+    c.rng_states = uniforms ? nullptr : rng_states;
+    c.out_tokens = out_tokens;
+    c.out_accepted = out_accepted;
+    c.out_status = out_status;
+    return c;
+}
+
+bool misaligned(const void *p, size_t bytes) {
+    return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) != 0;
+}
+
+}  // namespace
+
+rsc_status rsc_verify(rsc_sampler *s, const rsc_draft_batch *x, const rsc_params *params,
+                      const float *d_uniforms, uint64_t *d_rng_states, void *d_workspace,
+                      size_t workspace_bytes, uint32_t *d_out_tokens, uint32_t *d_out_accepted,
+                      int32_t *d_out_status, void *stream) {
+    rsc_status st = check_verify(s, x, d_out_tokens, d_out_accepted, d_out_status);
+    if (st != RSC_OK) return st;
+    if (!params) return RSC_ERR_INVALID_ARGUMENT;
+    if (x->vocab > kMaxVocab) return RSC_ERR_VOCAB_TOO_LARGE;
+    const rsc::CallParams cp = make_params(*params, x->vocab, d_uniforms, d_rng_states);
+    const bool greedy = cp.argmax_branch;
+    if (!cp.normal_scale || (!greedy && (!(params->temperature > 0.0f) || cp.topk_active || cp.topp_active)))
+        return RSC_ERR_INVALID_ARGUMENT;
+    if (x->n_seqs == 0) return RSC_OK;
+    if (x->vocab == 0) return RSC_ERR_INVALID_SHAPE;
+    const float *draft = greedy ? nullptr : x->d_draft;
+    if (!x->d_target || misaligned(x->d_target, 4) || misaligned(draft, 4))
+        return RSC_ERR_INVALID_ARGUMENT;
+    if (x->max_drafts > 0 && x->target_row_stride < x->vocab) return RSC_ERR_INVALID_SHAPE;
+    if (x->n_seqs > 1 && x->target_seq_stride < x->vocab) return RSC_ERR_INVALID_SHAPE;
+    if (draft && ((x->max_drafts > 1 && x->draft_row_stride < x->vocab) ||
+                  (x->n_seqs > 1 && x->max_drafts > 0 && x->draft_seq_stride < x->vocab)))
+        return RSC_ERR_INVALID_SHAPE;
+    if (!greedy && !d_uniforms && !d_rng_states) return RSC_ERR_INVALID_ARGUMENT;
+    if (!d_workspace || misaligned(d_workspace, 16) ||
+        workspace_bytes < rsc::verify_workspace_bytes(x->n_seqs, x->max_drafts, x->vocab))
+        return RSC_ERR_INVALID_ARGUMENT;
+    rsc::VerifyCall c = verify_call(*x, d_uniforms, d_rng_states, d_out_tokens, d_out_accepted, d_out_status);
+    c.vocab = static_cast<uint32_t>(x->vocab);
+    c.scale = cp.scale;
+    c.target = x->d_target;
+    c.target_seq_stride = x->target_seq_stride;
+    c.target_row_stride = x->target_row_stride;
+    c.draft = x->max_drafts > 0 ? draft : nullptr;
+    c.draft_seq_stride = x->draft_seq_stride;
+    c.draft_row_stride = x->draft_row_stride;
+    c.row_parts = d_workspace;
+    DeviceGuard guard(s->device);
+    return cuda_status(rsc::launch_verify(c, greedy, s->num_sms, &s->launches,
+                                          static_cast<cudaStream_t>(stream)));
+}
+
+rsc_status rsc_verify_survivors(rsc_sampler *s, const rsc_draft_batch *x,
+                                const rsc_survivor_records *target,
+                                const rsc_survivor_records *draft, const float *d_uniforms,
+                                uint64_t *d_rng_states, uint32_t *d_out_tokens,
+                                uint32_t *d_out_accepted, int32_t *d_out_status, void *stream) {
+    rsc_status st = check_verify(s, x, d_out_tokens, d_out_accepted, d_out_status);
+    if (st != RSC_OK) return st;
+    if (!target) return RSC_ERR_INVALID_ARGUMENT;
+    if (x->n_seqs == 0) return RSC_OK;
+    if (x->max_drafts == 0) draft = nullptr;
+    if (!d_uniforms && !d_rng_states) return RSC_ERR_INVALID_ARGUMENT;
+    rsc::VerifyCall c = verify_call(*x, d_uniforms, d_rng_states, d_out_tokens, d_out_accepted, d_out_status);
+    const rsc_survivor_records *given[2] = {target, draft};
+    rsc::VerifyRecords *taken[2] = {&c.target_rec, &c.draft_rec};
+    for (int k = 0; k < 2; ++k) {
+        if (!given[k]) continue;
+        if (!given[k]->d_n || !given[k]->d_ids || !given[k]->d_probs || given[k]->cap == 0 ||
+            given[k]->cap > kMaxVocab)
+            return RSC_ERR_INVALID_ARGUMENT;
+        *taken[k] = rsc::VerifyRecords{given[k]->d_n, given[k]->d_ids, given[k]->d_probs,
+                                       given[k]->d_status, given[k]->cap};
+    }
+    DeviceGuard guard(s->device);
+    ++s->launches;
+    return cuda_status(rsc::launch_verify_records(c, static_cast<cudaStream_t>(stream)));
+}
+
 uint64_t rsc_launch_count(const rsc_sampler *s) { return s && s->alive ? s->launches : 0; }
 
 rsc_status rsc_debug_hold_scratch(rsc_sampler *s, int hold, void *stream) {

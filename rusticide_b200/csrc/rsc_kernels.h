@@ -205,6 +205,45 @@ cudaError_t launch_expf(const float *x, float *y, size_t n, cudaStream_t stream)
 cudaError_t launch_rng_seed(const uint64_t *seeds, uint64_t *states, size_t rows,
                             cudaStream_t stream);
 
+// Verification of drafted tokens (verify.cu).
+constexpr uint32_t kVerifyMaxParts = 16;  // CTAs a row is spread over
+constexpr uint64_t kVerifyMaxRows = uint64_t{1} << 27;
+
+// Survivor records of consecutive rows (rsc_survivor_records in the C header).
+struct VerifyRecords {
+    const uint32_t *n = nullptr;
+    const uint32_t *ids = nullptr;
+    const float *probs = nullptr;
+    const int32_t *status = nullptr;
+    size_t cap = 0;
+};
+
+struct VerifyCall {
+    uint32_t n_seqs, max_drafts, vocab;
+    float scale;
+    const float *target;  // row i of sequence b at target + b * target_seq_stride + i * target_row_stride
+    size_t target_seq_stride, target_row_stride;
+    const float *draft;   // nullable
+    size_t draft_seq_stride, draft_row_stride;
+    VerifyRecords target_rec, draft_rec;  // instead of logits (verify_records)
+    const uint32_t *draft_tokens;         // [n_seqs][max_drafts]
+    const int32_t *n_draft;               // nullable
+    const float *uniforms;                // [n_seqs][max_drafts + 1], nullable
+    uint64_t *rng_states;                 // [n_seqs], nullable
+    void *row_parts;                      // verify_workspace_bytes
+    uint32_t parts;                       // set by launch_verify
+    uint32_t *out_tokens;                 // [n_seqs][max_drafts + 1]
+    uint32_t *out_accepted;               // [n_seqs]
+    int32_t *out_status;                  // [n_seqs]
+};
+
+size_t verify_workspace_bytes(size_t n_seqs, size_t max_drafts, size_t vocab);
+// Two launches (rows, then decisions and draws); *launches counts them.
+// vocab > 0, n_seqs > 0.
+cudaError_t launch_verify(const VerifyCall &c, bool greedy, int num_sms, uint64_t *launches,
+                          cudaStream_t stream);
+cudaError_t launch_verify_records(const VerifyCall &c, cudaStream_t stream);
+
 // Shared-memory bytes of the streaming kernel (for occupancy queries).
 size_t stream_topk_smem_bytes();
 

@@ -391,6 +391,165 @@ class Engine:
                                        _ptr(probs), _stream_ptr(self.device)), "rsc_shard_merge")
         return ids, status, probs
 
+    # -- verification of drafted tokens ---------------------------------------
+    def _want(self, t: torch.Tensor, what: str, dtype: torch.dtype, shape: tuple) -> int:
+        """The address of a dense argument of this type and shape on the engine's device."""
+        if t.device != self.device:
+            raise ValueError(f"{what} on {t.device}, engine on {self.device}")
+        if t.dtype != dtype:
+            raise TensorError(str(dtype).replace("torch.", ""), str(t.dtype).replace("torch.", ""))
+        if t.shape != shape:
+            raise InvalidShape(list(t.shape))
+        if not t.is_contiguous():
+            raise ValueError(f"{what} must be contiguous")
+        return t.data_ptr()
+
+    def _rows_3d(self, t: torch.Tensor, what: str, shape: tuple) -> tuple[int, int, int]:
+        """(address, sequence stride, row stride) of [sequences, rows, vocab] f32 logits whose rows
+        are contiguous; the strides may be larger than dense ones, and in either order."""
+        if t.device != self.device:
+            raise ValueError(f"{what} on {t.device}, engine on {self.device}")
+        if t.dtype != torch.float32:
+            raise TensorError("F32", str(t.dtype).replace("torch.", "").upper())
+        if t.shape != shape:
+            raise InvalidShape(list(t.shape))
+        seqs, rows, vocab = shape
+        ss, rs, es = t.stride()
+        if vocab > 1 and es != 1 and t.numel() > 0:
+            raise ValueError("logit rows must be contiguous")
+        # A dimension of one element has no stride to go by.
+        rs = rs if rows > 1 else vocab
+        return t.data_ptr(), ss if seqs > 1 else rows * rs, rs
+
+    def _draft_batch(self, target_logits, draft_tokens: torch.Tensor, draft_logits, n_draft):
+        if draft_tokens.dim() != 2:
+            raise InvalidShape(list(draft_tokens.shape))
+        seqs, drafts = draft_tokens.shape
+        x = _lib.RscDraftBatch()
+        x.n_seqs, x.max_drafts = seqs, drafts
+        x.d_draft_tokens = self._want(draft_tokens, "draft_tokens", torch.int32, (seqs, drafts))
+        if n_draft is not None:
+            x.d_n_draft = self._want(n_draft, "n_draft", torch.int32, (seqs,))
+        if target_logits is not None:
+            if target_logits.dim() != 3:
+                raise InvalidShape(list(target_logits.shape))
+            x.vocab = vocab = target_logits.shape[2]
+            x.d_target, x.target_seq_stride, x.target_row_stride = self._rows_3d(
+                target_logits, "target_logits", (seqs, drafts + 1, vocab))
+            if draft_logits is not None and drafts > 0:
+                x.d_draft, x.draft_seq_stride, x.draft_row_stride = self._rows_3d(
+                    draft_logits, "draft_logits", (seqs, drafts, vocab))
+        return x
+
+    def _verify_draws(self, seqs: int, drafts: int, uniforms, rng_states):
+        u = None if uniforms is None else self._want(uniforms, "uniforms", torch.float32,
+                                                     (seqs, drafts + 1))
+        st = None if rng_states is None else self._want(rng_states, "rng_states", torch.int64, (seqs,))
+        return u, st
+
+    def _verify_outputs(self, seqs: int, drafts: int, out):
+        if out is None:
+            dev = self.device
+            return (torch.empty((seqs, drafts + 1), dtype=torch.int32, device=dev),
+                    torch.empty(seqs, dtype=torch.int32, device=dev),
+                    torch.empty(seqs, dtype=torch.int32, device=dev))
+        for t, what, shape in zip(out, ("tokens", "accepted", "status"),
+                                  ((seqs, drafts + 1), (seqs,), (seqs,))):
+            self._want(t, f"out {what}", torch.int32, shape)
+        return out
+
+    def verify(self, target_logits: torch.Tensor, draft_tokens: torch.Tensor,
+               params: SamplingParams, uniforms: Optional[torch.Tensor] = None,
+               rng_states: Optional[torch.Tensor] = None,
+               draft_logits: Optional[torch.Tensor] = None,
+               n_draft: Optional[torch.Tensor] = None, survivor_cap: Optional[int] = None, out=None):
+        """Verifies drafted tokens against the target model's logits, so that the output is
+        distributed as if every token had been sampled from the target with `params`.
+
+        target_logits [sequences, drafts + 1, vocab] f32, draft_tokens [sequences, drafts] int32,
+        draft_logits [sequences, drafts, vocab] f32 (None: the drafts have no distribution, as
+        tokens looked up in the prompt), n_draft [sequences] int32 (None: all of them), uniforms
+        [sequences, drafts + 1] f32 in [0, 1) or rng_states [sequences]. Returns (tokens
+        [sequences, drafts + 1] int32, accepted [sequences], status [sequences]): the accepted
+        tokens, one more, then -1; see rsc_verify in the C header.
+
+        With top-k and top-p off this is rsc_verify. A filtered distribution is verified from its
+        survivor records (rsc_sample_ex, then rsc_verify_survivors) of survivor_cap slots a row
+        (None: top_k plus 24 for ties, or the vocabulary when top-k is off); a row with more
+        survivors gives its sequence status RSC_ROW_INTERNAL."""
+        x = self._draft_batch(target_logits, draft_tokens, draft_logits, n_draft)
+        seqs, drafts, vocab = x.n_seqs, x.max_drafts, x.vocab
+        argmax = params.temperature == 0 or params.top_k == 1
+        if not argmax and (0 < params.top_k < vocab or params.top_p < 1.0):
+            if uniforms is None and rng_states is None:
+                check(_lib.RSC_ERR_INVALID_ARGUMENT, "rsc_verify_survivors")
+            if survivor_cap is None:
+                survivor_cap = params.top_k + _lib.RSC_SHARD_TIE_CAP if 0 < params.top_k < vocab else vocab
+            target = self._records(target_logits, params, min(survivor_cap, vocab))
+            draft = None
+            if draft_logits is not None and drafts > 0:
+                draft = self._records(draft_logits, params, min(survivor_cap, vocab))
+            return self.verify_survivors(target, draft_tokens, uniforms=uniforms,
+                                         rng_states=rng_states, draft=draft, n_draft=n_draft, out=out)
+        u, st = self._verify_draws(seqs, drafts, uniforms, rng_states)
+        tokens, accepted, status = self._verify_outputs(seqs, drafts, out)
+        nbytes = self.lib.rsc_verify_workspace_bytes(seqs, drafts, vocab)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        check(self.lib.rsc_verify(self._h, ctypes.byref(x), ctypes.byref(params.to_c()), u, st,
+                                  work.data_ptr(), nbytes, tokens.data_ptr(), accepted.data_ptr(),
+                                  status.data_ptr(), _stream_ptr(self.device)), "rsc_verify")
+        return tokens, accepted, status
+
+    def _records(self, logits: torch.Tensor, params: SamplingParams, cap: int):
+        """Survivor records (n, ids, probs, status) of [sequences, rows, vocab] logits."""
+        flat = logits.reshape(-1, logits.shape[2])
+        rows, vocab, stride = self._check_rows(flat)
+        n = torch.empty(rows, dtype=torch.int32, device=self.device)
+        ids = torch.empty((rows, cap), dtype=torch.int32, device=self.device)
+        probs = torch.empty((rows, cap), dtype=torch.float32, device=self.device)
+        token, status, _ = self._outputs(rows, False)
+        unused = torch.zeros(rows, dtype=torch.float32, device=self.device)  # the token is not kept
+        ex = _lib.RscSampleExtras(n.data_ptr(), ids.data_ptr(), cap, probs.data_ptr(), None, None, None)
+        check(self.lib.rsc_sample_ex(self._h, flat.data_ptr(), rows, vocab, stride,
+                                     ctypes.byref(params.to_c()), unused.data_ptr(), None,
+                                     token.data_ptr(), status.data_ptr(), None, ctypes.byref(ex),
+                                     _stream_ptr(self.device)), "rsc_sample_ex")
+        return n, ids, probs, status
+
+    def _record_struct(self, record, what: str, rows: int):
+        n, ids, probs = record[:3]
+        status = record[3] if len(record) > 3 else None
+        if ids.dim() != 2:
+            raise InvalidShape(list(ids.shape))
+        cap = ids.shape[1]
+        return _lib.RscSurvivorRecords(
+            self._want(n, f"{what} n", torch.int32, (rows,)),
+            self._want(ids, f"{what} ids", torch.int32, (rows, cap)),
+            self._want(probs, f"{what} probs", torch.float32, (rows, cap)),
+            None if status is None else self._want(status, f"{what} status", torch.int32, (rows,)), cap)
+
+    def verify_survivors(self, target, draft_tokens: torch.Tensor,
+                         uniforms: Optional[torch.Tensor] = None,
+                         rng_states: Optional[torch.Tensor] = None, draft=None,
+                         n_draft: Optional[torch.Tensor] = None, out=None):
+        """rsc_verify_survivors: `verify` with each distribution given as a survivor record, a tuple
+        (n [rows], ids [rows, cap], probs [rows, cap]) and optionally status [rows], as sample_ex
+        returns them: the target's over sequences * (drafts + 1) rows, the draft's (None: no
+        distribution) over sequences * drafts rows."""
+        x = self._draft_batch(None, draft_tokens, None, n_draft)
+        seqs, drafts = x.n_seqs, x.max_drafts
+        u, st = self._verify_draws(seqs, drafts, uniforms, rng_states)
+        t = self._record_struct(target, "target", seqs * (drafts + 1))
+        d = None
+        if draft is not None and drafts > 0:
+            d = ctypes.byref(self._record_struct(draft, "draft", seqs * drafts))
+        tokens, accepted, status = self._verify_outputs(seqs, drafts, out)
+        check(self.lib.rsc_verify_survivors(self._h, ctypes.byref(x), ctypes.byref(t), d, u, st,
+                                            tokens.data_ptr(), accepted.data_ptr(),
+                                            status.data_ptr(), _stream_ptr(self.device)),
+              "rsc_verify_survivors")
+        return tokens, accepted, status
+
     # -- LM head with the sampler fused into its epilogue ----------------------
     @staticmethod
     def _lmhead_args(hidden: torch.Tensor, weight: torch.Tensor):
@@ -522,6 +681,24 @@ class Sampler:
         ids, status, _ = self._engine.sample_with_temp(row, temperature, rng_states=self._state,
                                                        want_probs=False)
         return self._result(ids, status)
+
+    def verify(self, target_logits: torch.Tensor, draft_tokens: Sequence[int],
+               params: SamplingParams, draft_logits: Optional[torch.Tensor] = None) -> list[int]:
+        """Verifies this stream's drafted tokens: target_logits [drafts + 1, vocab], draft_logits
+        [drafts, vocab] or None (see Engine.verify). Returns the tokens to append: the accepted
+        ones and one more. The generator advances by one draw per test and one for the last token
+        (greedy parameters draw nothing)."""
+        if target_logits.dim() != 2 or target_logits.shape[0] != len(draft_tokens) + 1:
+            raise InvalidShape(list(target_logits.shape))
+        drafts = torch.tensor([[int(t) for t in draft_tokens]], dtype=torch.int64).to(torch.int32)
+        q = None if draft_logits is None else draft_logits.to(self.device)[None]
+        tokens, accepted, status = self._engine.verify(
+            target_logits.to(self.device)[None], drafts.to(self.device), params,
+            rng_states=self._state, draft_logits=q)
+        err = row_error(int(status[0].item()))
+        if err is not None:
+            raise err
+        return [int(t) & 0xFFFFFFFF for t in tokens[0, :int(accepted[0].item()) + 1].tolist()]
 
     def penalize(self, logits: torch.Tensor, tokens: Sequence[int], penalty: float) -> None:
         """Sampler::penalize (src/sampler.rs:107-109), in place on a device row."""

@@ -1,0 +1,454 @@
+"""Draft verification on the GPU against the binary64 form of verify_ref.py. Tokens, accepted counts
+and statuses are whole numbers and have to be equal: the device decides as exact arithmetic does up
+to 1e-13 relative, and of the at most 1e4 decisions below, each with uniforms that are multiples of
+2^-24 or 2^-32, none is expected within that of an edge."""
+
+import numpy as np
+import pytest
+import torch
+
+from rusticide_b200 import Sampler, SamplingParams, _lib, engine
+
+from . import verify_ref as R
+
+pytestmark = pytest.mark.gpu
+
+FULL = SamplingParams(1.0, 0, 1.0)
+
+
+def case(b, d, v, seed, draft=True, spread=2.0, noise=0.5):
+    """Logits, drafts and uniforms of a batch; tokens drawn from the draft's rows."""
+    rng = np.random.default_rng(seed)
+    x = (rng.normal(size=(b, d + 1, v)) * spread).astype(np.float32)
+    y = (x[:, :d] + noise * rng.normal(size=(b, d, v))).astype(np.float32)
+    g = rng.gumbel(size=(b, d, v))
+    t = (y + g).argmax(2).astype(np.int32) if d else np.zeros((b, 0), np.int32)
+    u = rng.random((b, d + 1), dtype=np.float32)
+    return x, (y if draft else None), t, u
+
+
+def dev(a):
+    return None if a is None else torch.from_numpy(np.ascontiguousarray(a)).cuda()
+
+
+def run(x, y, t, u, params=FULL, n=None, **kw):
+    out = engine(0).verify(dev(x), dev(t), params, uniforms=dev(u), draft_logits=dev(y),
+                           n_draft=dev(n), **kw)
+    torch.cuda.synchronize()
+    return [o.cpu().numpy() for o in out]
+
+
+def same(got, want):
+    for g, w, what in zip(got, want, ("tokens", "accepted", "status")):
+        np.testing.assert_array_equal(g, w, err_msg=what)
+
+
+@pytest.mark.parametrize("v", [1, 2, 3, 31, 33, 1000, 2049, 4097, 50001])
+@pytest.mark.parametrize("b,d", [(1, 1), (3, 4), (2, 0), (1, 20)])
+@pytest.mark.parametrize("draft", [True, False])
+def test_sizes(b, d, v, draft):
+    x, y, t, u = case(b, d, v, seed=b * 1000 + d * 100 + v, draft=draft)
+    same(run(x, y, t, u), R.verify_batch(x, y, t, None, u, 1.0))
+
+
+@pytest.mark.parametrize("temperature", [0.25, 0.8, 1.3, 7.0])
+@pytest.mark.parametrize("draft", [True, False])
+def test_ragged_batches(temperature, draft):
+    b, d, v = 40, 6, 3001
+    x, y, t, u = case(b, d, v, seed=5, draft=draft)
+    n = np.random.default_rng(6).integers(-2, d + 3, size=b).astype(np.int32)
+    want = R.verify_batch(x, y, t, n, u, temperature)
+    # What lies behind a sequence's drafts is not looked at.
+    for i in range(b):
+        k = int(np.clip(n[i], 0, d))
+        x[i, k + 1:] = np.nan
+        t[i, k:] = -7
+        if draft:
+            y[i, k:] = np.inf
+    same(run(x, y, t, u, SamplingParams(temperature, 0, 1.0), n=n), want)
+    # More sequences than the GPU has SMs: one CTA draws for a sequence.
+    reps = 10
+    big = [np.concatenate([a] * reps) if a is not None else None for a in (x, y, t, u, n)]
+    got = run(*big[:4], SamplingParams(temperature, 0, 1.0), n=big[4])
+    same(got, [np.concatenate([w] * reps) for w in want])
+
+
+def test_flat_rows_are_drawn_exactly():
+    """Equal weights over a large vocabulary: the drawn index is floor(u * V), whose neighbours are
+    1 / V away, far below binary32's reach in a running sum of this length."""
+    b, v = 64, 151936
+    x = np.zeros((b, 1, v), np.float32)
+    u = np.random.default_rng(0).random((b, 1), dtype=np.float32)
+    got = run(x, None, np.zeros((b, 0), np.int32), u)
+    edge = u[:, 0].astype(np.float64) * v
+    assert np.abs(edge - np.round(edge)).min() > 1e-4
+    np.testing.assert_array_equal(got[0][:, 0], np.floor(edge).astype(np.int32))
+
+
+def test_residual_over_a_large_flat_vocabulary():
+    b, d, v = 4, 1, 151936
+    x, y, t, u = case(b, d, v, seed=9, spread=0.5, noise=0.5)
+    u[:, 0] = np.float32(1 - 2.0 ** -24)  # refuse whatever can be refused
+    want = R.verify_batch(x, y, t, None, u, 1.0)
+    assert (want[1] == 0).any()
+    same(run(x, y, t, u), want)
+
+
+def test_equal_distributions_accept_every_token():
+    """p = q: u < 1 accepts, by a margin of 2^-24 that the binary32 sums cannot see."""
+    b, d, v = 5, 6, 20011
+    x, _, t, u = case(b, d, v, seed=11)
+    y = x[:, :d].copy()
+    u[:, :d] = np.float32(1 - 2.0 ** -24)
+    got = run(x, y, t, u)
+    same(got, R.verify_batch(x, y, t, None, u, 1.0))
+    assert (got[1] == d).all()
+
+
+def test_edges_of_a_test():
+    """u exactly at p / q refuses (the test is strict); one step below accepts."""
+    v = 4
+    x = np.log(np.array([1, 2, 4, 1], np.float64) / 8).astype(np.float32)
+    x = np.zeros((1, 2, v), np.float32)          # p = 1/4 each, exactly
+    y = np.full((1, 1, v), -np.inf, np.float32)
+    y[0, 0, 2] = 3.0                             # q = 1 at token 2
+    t = np.array([[2]], np.int32)
+    for u0, accepted in ((0.25, 0), (np.nextafter(np.float32(0.25), np.float32(0)), 1), (0.0, 1)):
+        u = np.array([[u0, 0.5]], np.float32)
+        for q in (y, None):
+            got = run(x, q, t, u)
+            assert got[1][0] == accepted
+            same(got, R.verify_batch(x, q, t, None, u, 1.0))
+
+
+def test_masked_tokens_nan_and_infinities():
+    b, d, v = 12, 3, 777
+    x, y, t, u = case(b, d, v, seed=21)
+    rng = np.random.default_rng(22)
+    x[rng.random(x.shape) < 0.5] = -np.inf
+    y[rng.random(y.shape) < 0.5] = -np.inf
+    x[rng.random(x.shape) < 0.05] = np.nan
+    x[0, 0] = -np.inf                 # no distribution at the first test
+    x[1, 0, 5] = np.inf               # nor with a logit of +inf
+    y[2, 0] = np.nan                  # nor for the draft
+    y[3, 0, 7] = np.inf
+    x[4, 2] = -np.inf                 # needed only if two tokens pass
+    x[5, :, :] = -np.inf
+    x[5, :, 3] = 1.0                  # one token left: it is drawn
+    y[5, :, :] = -np.inf
+    y[5, :, 3] = 1.0
+    t[5] = 3
+    x[6] = np.finfo(np.float32).min   # masks of the type's lowest value
+    x[6, :, 9] = 0.0
+    x[7] = np.finfo(np.float32).max   # differences that leave binary32
+    x[7, :, ::2] = np.finfo(np.float32).min
+    t[8] = [v, v + 5, -1]             # outside the vocabulary
+    t[9, 0] = np.int32(2 ** 31 - 1)
+    y[10] = x[10, :d]                 # equal rows, a token outside both
+    x[10, 0, t[10, 0]] = y[10, 0, t[10, 0]] = -np.inf
+    for q in (y, None):
+        same(run(x, q, t, u), R.verify_batch(x, q, t, None, u, 1.0))
+
+
+@pytest.mark.parametrize("offset", [0, 1, 2, 3])
+def test_strides_and_alignment(offset):
+    b, d, v = 3, 2, 5003
+    x, y, t, u = case(b, d, v, seed=31)
+    want = R.verify_batch(x, y, t, None, u, 1.0)
+    eng = engine(0)
+
+    def spread(a, order):
+        """The values at `offset` floats into a wider allocation, sequences or rows slowest."""
+        s0, s1, _ = a.shape
+        pitch = v + 13 + offset
+        buf = torch.full((s0 * s1 * pitch + 8,), float("nan"), device="cuda")
+        strides = (s1 * pitch, pitch, 1) if order else (pitch, s0 * pitch, 1)
+        view = torch.as_strided(buf, a.shape, strides, offset)
+        view.copy_(torch.from_numpy(a))
+        return view
+
+    for order in (True, False):
+        out = eng.verify(spread(x, order), dev(t), FULL, uniforms=dev(u),
+                         draft_logits=spread(y, not order))
+        same([o.cpu().numpy() for o in out], want)
+
+
+@pytest.mark.parametrize("v", [1, 5, 4099, 151936])
+def test_greedy(v):
+    b, d = 9, 5
+    rng = np.random.default_rng(v)
+    x = rng.normal(size=(b, d + 1, v)).astype(np.float32)
+    x[1] = np.round(x[1])                       # ties: the last index counts
+    t = x[:, :d].argmax(2).astype(np.int32)
+    t[1] = v - 1 - x[1, :d, ::-1].argmax(1)
+    t[2, 2] = (t[2, 2] + 1) % v
+    t[3, 0] = -1
+    x[4, 1] = -np.inf
+    x[5, 2] = np.nan
+    x[6, :, 0] = np.inf                         # larger than any finite logit
+    n = np.array([d, d, d, d, d, d, d, 2, 0], np.int32)
+    want = R.greedy_batch(x, t, n)
+    y = np.full((b, d, v), np.nan, np.float32)  # not read
+    for params in (SamplingParams(0.0, 40, 0.9), SamplingParams(0.0, 0, 1.0)):
+        out = engine(0).verify(dev(x), dev(t), params, n_draft=dev(n), draft_logits=dev(y))
+        same([o.cpu().numpy() for o in out], want)
+    # The tokens are those of the greedy call on the same rows.
+    ids, _ = engine(0).greedy(dev(x).reshape(-1, v))
+    ids = ids.cpu().numpy().reshape(b, d + 1)
+    for i in range(b):
+        if want[2][i] == 0:
+            assert want[0][i, want[1][i]] == ids[i, want[1][i]]
+
+
+def test_top_k_of_one_is_greedy():
+    b, d, v = 4, 3, 999
+    x, y, t, u = case(b, d, v, seed=41)
+    t[:2] = x[:2, :d].argmax(2)
+    same(run(x, y, t, u, SamplingParams(0.7, 1, 0.9)), R.greedy_batch(x, t, None))
+
+
+def test_generator_states():
+    """Draws from per-sequence states equal the same draws given as uniforms, and a state advances
+    by what its sequence consumed."""
+    b, d, v = 30, 4, 2003
+    x, y, t, _ = case(b, d, v, seed=51)
+    x[3, 0] = -np.inf                     # no draw at all
+    x[4, d] = -np.inf                     # tests only, if all pass
+    seeds = list(range(100, 100 + b))
+    for draft in (y, None):
+        states = engine(0).rng_seed(torch.tensor(seeds))
+        got = [o.cpu().numpy() for o in engine(0).verify(
+            dev(x), dev(t), FULL, rng_states=states, draft_logits=dev(draft))]
+        for i in range(b):
+            u = R.wyrand_uniforms(seeds[i], d + 1)
+            row, acc, st, used = R.verify_one(
+                lambda k: R.softmax(R.scaled(x[i, k], 1.0)),
+                None if draft is None else lambda k: R.softmax(R.scaled(draft[i, k], 1.0)),
+                t[i], d, u, lambda k: u[k])
+            assert got[0][i, :len(row)].tolist() == [int(r) for r in row]
+            assert (got[0][i, len(row):] == -1).all()
+            assert (got[1][i], got[2][i]) == (acc, st)
+            state = (seeds[i] + used * 0x2d358dccaa6c78a5) & ((1 << 64) - 1)
+            assert int(states[i]) & ((1 << 64) - 1) == state
+
+
+def test_a_sequence_does_not_depend_on_its_batch():
+    b, d, v = 17, 5, 9001
+    x, y, t, u = case(b, d, v, seed=61)
+    whole = run(x, y, t, u)
+    for i in range(b):
+        one = run(x[i:i + 1], y[i:i + 1], t[i:i + 1], u[i:i + 1])
+        same(one, [w[i:i + 1] for w in whole])
+
+
+def test_output_distribution():
+    """Over many sequences of one position the first token follows p. With N = 200000 draws a share
+    is off by more than 6 standard deviations, 6 sqrt(p (1 - p) / N), with odds below 1e-8."""
+    n, v = 200000, 6
+    rng = np.random.default_rng(71)
+    x = rng.normal(size=(1, 2, v)).astype(np.float32)
+    y = rng.normal(size=(1, 1, v)).astype(np.float32)
+    p, q = R.softmax(x[0, 0]), R.softmax(y[0, 0])
+    t = rng.choice(v, size=(n, 1), p=q).astype(np.int32)
+    u = rng.random((n, 2), dtype=np.float32)
+    out = engine(0).verify(dev(x).expand(n, 2, v).contiguous(), dev(t), FULL, uniforms=dev(u),
+                           draft_logits=dev(y).expand(n, 1, v).contiguous())
+    share = np.bincount(out[0][:, 0].cpu().numpy(), minlength=v) / n
+    assert (np.abs(share - p) < 6 * np.sqrt(p * (1 - p) / n)).all()
+
+
+def test_streams_graphs_and_reused_outputs():
+    b, d, v = 6, 3, 30011
+    sets = [case(b, d, v, seed=81 + k) for k in range(2)]
+    want = [R.verify_batch(*s[:3], None, s[3], 1.0) for s in sets]
+    ins = [[dev(a) for a in s] for s in sets]
+    eng = engine(0)
+    torch.cuda.synchronize()
+    # Two calls in flight on two streams.
+    streams = [torch.cuda.Stream() for _ in sets]
+    outs = []
+    for s, (x, y, t, u) in zip(streams, ins):
+        with torch.cuda.stream(s):
+            outs.append(eng.verify(x, t, FULL, uniforms=u, draft_logits=y))
+    torch.cuda.synchronize()
+    for o, w in zip(outs, want):
+        same([a.cpu().numpy() for a in o], w)
+    # Two captured calls, replayed in turn, with outputs and inputs that are the caller's.
+    graphs = []
+    for x, y, t, u in ins:
+        out = tuple(torch.empty_like(o) for o in outs[0])
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = eng.verify(x, t, FULL, uniforms=u, draft_logits=y, out=out)
+        assert all(a is b_ for a, b_ in zip(got, out))
+        graphs.append((g, out))
+    for _ in range(3):
+        for g, _ in graphs:
+            g.replay()
+    torch.cuda.synchronize()
+    for (_, o), w in zip(graphs, want):
+        same([a.cpu().numpy() for a in o], w)
+    # New inputs in the captured buffers.
+    for a, b_ in zip(ins[0], ins[1]):
+        a.copy_(b_)
+    graphs[0][0].replay()
+    torch.cuda.synchronize()
+    same([a.cpu().numpy() for a in graphs[0][1]], want[1])
+
+
+# ---------------------------------------------------------------------------
+# Survivor records
+# ---------------------------------------------------------------------------
+def records(rng, rows, vocab, cap, empty=False):
+    n = rng.integers(0 if empty else 1, min(cap, vocab) + 1, size=rows).astype(np.int32)
+    ids = np.full((rows, cap), -1, np.int32)
+    probs = np.full((rows, cap), np.nan, np.float32)
+    for r in range(rows):
+        k = int(n[r])
+        ids[r, :k] = np.sort(rng.choice(vocab, size=k, replace=False))
+        w = rng.random(k) ** 3 + 1e-3
+        probs[r, :k] = (w / w.sum()).astype(np.float32) if k else 0
+    return n, ids, probs
+
+
+@pytest.mark.parametrize("b,d,vocab,cap", [(1, 1, 4, 1), (1, 4, 40, 16), (50, 3, 64, 40),
+                                           (20, 9, 300, 152), (3, 2, 5000, 1500), (5, 0, 30, 8)])
+@pytest.mark.parametrize("with_draft", [True, False])
+def test_records(b, d, vocab, cap, with_draft):
+    rng = np.random.default_rng(b * 100 + d + cap)
+    target = records(rng, b * (d + 1), vocab, cap)
+    draft = records(rng, b * d, vocab, cap) if with_draft else None
+    t = rng.integers(0, vocab, size=(b, d)).astype(np.int32)
+    for i in range(b):  # most tokens come from the target's list, some from neither
+        for k in range(d):
+            if rng.random() < 0.8:
+                row = i * (d + 1) + k
+                t[i, k] = target[1][row, rng.integers(0, target[0][row])]
+    u = rng.random((b, d + 1), dtype=np.float32)
+    n = rng.integers(0, d + 1, size=b).astype(np.int32)
+    out = engine(0).verify_survivors([dev(a) for a in target], dev(t), uniforms=dev(u),
+                                     draft=None if draft is None else [dev(a) for a in draft],
+                                     n_draft=dev(n))
+    same([o.cpu().numpy() for o in out], R.verify_records(target, draft, vocab, t, n, u))
+
+
+def test_records_that_hold_no_distribution():
+    rng = np.random.default_rng(1)
+    b, d, vocab, cap = 6, 2, 50, 8
+    target, draft = records(rng, b * (d + 1), vocab, cap), records(rng, b * d, vocab, cap)
+    t = np.tile(target[1].reshape(b, d + 1, cap)[:, :d, 0], 1).astype(np.int32)
+    u = np.zeros((b, d + 1), np.float32)  # u = 0 accepts every listed token
+    status = np.zeros(b * (d + 1), np.int32)
+    target[0][0] = 0                        # sequence 0, row 0: empty
+    target[0][1 * 3 + 1] = cap + 1          # sequence 1, row 1: more survivors than slots
+    status[2 * 3 + 2] = 0x102               # sequence 2, last row: a status, with a flag above it
+    draft[0][3 * 2 + 1] = cap + 3           # sequence 3, draft row 1
+    target[2][4 * 3 + 2, :] = 0.0           # sequence 4, last row: no weight
+    out = engine(0).verify_survivors([dev(a) for a in target] + [dev(status)], dev(t),
+                                     uniforms=dev(u), draft=[dev(a) for a in draft])
+    tokens, accepted, st = [o.cpu().numpy() for o in out]
+    assert accepted.tolist() == [0, 1, 2, 1, 2, 2]
+    assert st.tolist() == [_lib.RSC_ROW_NO_VALID_TOKENS, _lib.RSC_ROW_INTERNAL, 2,
+                           _lib.RSC_ROW_INTERNAL, _lib.RSC_ROW_NO_VALID_TOKENS, 0]
+    for i in range(5):
+        assert tokens[i, :accepted[i]].tolist() == t[i, :accepted[i]].tolist()
+        assert (tokens[i, accepted[i]:] == -1).all()
+
+
+@pytest.mark.parametrize("params", [SamplingParams(0.8, 40, 0.95), SamplingParams(1.0, 0, 0.9),
+                                    SamplingParams(1.2, 100, 1.0)])
+@pytest.mark.parametrize("draft", [True, False])
+def test_filtered_parameters(params, draft):
+    """Engine.verify with top-k and top-p: the distributions are the sampler's own survivors."""
+    b, d, v = 8, 4, 3001
+    x, y, t, u = case(b, d, v, seed=91, draft=draft, spread=3.0)
+    eng = engine(0)
+
+    def survivors(a):
+        rows = a.reshape(-1, v)
+        out = eng.sample_ex(dev(rows), params, uniforms=torch.zeros(len(rows), device="cuda"),
+                            survivor_cap=v)
+        return [o.cpu().numpy() for o in (out[3], out[4], out[5])]
+
+    want = R.verify_records(survivors(x), survivors(y) if draft else None, v, t, None, u)
+    same(run(x, y, t, u, params), want)
+    states = eng.rng_seed(torch.arange(b))
+    st0 = states.clone()
+    out = eng.verify(dev(x), dev(t), params, rng_states=states,
+                     draft_logits=dev(y) if draft else None)
+    u2 = np.zeros((b, d + 1), np.float32)
+    for i in range(b):  # the last draw takes the uniform behind the tests
+        us = R.wyrand_uniforms(int(st0[i]), d + 1)
+        u2[i, :d] = us[:d]
+        acc = int(out[1][i])
+        u2[i, d] = us[acc + (acc < d)]
+    same([o.cpu().numpy() for o in out],
+         R.verify_records(survivors(x), survivors(y) if draft else None, v, t, None, u2))
+
+
+def test_sampler_verify_follows_the_generator():
+    v, d = 500, 3
+    x, y, t, _ = case(1, d, v, seed=101)
+    s = Sampler(7)
+    first = s.verify(dev(x[0]), t[0].tolist(), FULL, draft_logits=dev(y[0]))
+    u = R.wyrand_uniforms(7, 2 * (d + 1))
+    row, _, _, used = R.verify_one(lambda k: R.softmax(x[0, k]), lambda k: R.softmax(y[0, k]),
+                                   t[0], d, u, lambda k: u[k])
+    assert first == [int(r) for r in row]
+    second = s.verify(dev(x[0]), t[0].tolist(), FULL, draft_logits=dev(y[0]))
+    row, _, _, _ = R.verify_one(lambda k: R.softmax(x[0, k]), lambda k: R.softmax(y[0, k]), t[0],
+                                d, u[used:], lambda k: u[used + k])
+    assert second == [int(r) for r in row]
+    assert s.verify(dev(x[0, :1]), [], SamplingParams(0.0)) == [int(x[0, 0].argmax())]
+    assert len(s.verify(dev(x[0]), t[0].tolist(), SamplingParams())) >= 1
+
+
+@pytest.mark.parametrize("params", [SamplingParams(-1.0, 0, 1.0), SamplingParams(float("inf"), 0, 1.0),
+                                    SamplingParams(float("nan"), 0, 1.0), SamplingParams(1e-45, 0, 1.0)])
+def test_parameters_without_a_distribution_are_refused(params):
+    x, y, t, u = case(1, 1, 8, seed=1)
+    with pytest.raises(_lib.RscError) as e:
+        run(x, y, t, u, params)
+    assert e.value.code == _lib.RSC_ERR_INVALID_ARGUMENT
+
+
+def test_refusals_of_the_library():
+    import ctypes
+    eng = engine(0)
+    x, y, t, u = (dev(a) for a in case(2, 2, 64, seed=1))
+    lib, work = eng.lib, torch.empty(1 << 16, dtype=torch.uint8, device="cuda")
+    o = torch.empty(64, dtype=torch.int32, device="cuda")
+
+    def call(params=FULL, uniforms=u.data_ptr(), states=None, wptr=work.data_ptr(), wbytes=1 << 16,
+             out=o.data_ptr(), **fields):
+        b = _lib.RscDraftBatch(2, 2, 64, x.data_ptr(), 3 * 64, 64, y.data_ptr(), 2 * 64, 64,
+                               t.data_ptr(), None)
+        for k, v in fields.items():
+            setattr(b, k, v)
+        c = params.to_c()
+        return lib.rsc_verify(eng.handle, ctypes.byref(b), ctypes.byref(c), uniforms, states, wptr,
+                              wbytes, out, out, out, None)
+
+    assert call() == _lib.RSC_OK
+    assert call(n_seqs=0, d_target=None) == _lib.RSC_OK
+    arg, shape = _lib.RSC_ERR_INVALID_ARGUMENT, _lib.RSC_ERR_INVALID_SHAPE
+    assert call(SamplingParams(1.0, 40, 1.0)) == arg        # a filtered distribution
+    assert call(SamplingParams(1.0, 0, 0.9)) == arg
+    assert call(uniforms=None) == arg
+    assert call(wbytes=16) == arg
+    assert call(wptr=None) == arg
+    assert call(wptr=work.data_ptr() + 4) == arg
+    assert call(out=None) == arg
+    assert call(d_target=None) == arg
+    assert call(d_target=x.data_ptr() + 1) == arg
+    assert call(d_draft=y.data_ptr() + 2) == arg
+    assert call(d_draft_tokens=None) == arg
+    assert call(vocab=0) == shape
+    assert call(target_row_stride=63) == shape
+    assert call(target_seq_stride=63) == shape
+    assert call(draft_row_stride=0) == shape
+    assert call(draft_seq_stride=0) == shape
+    assert call(vocab=1 << 31) == _lib.RSC_ERR_VOCAB_TOO_LARGE
+    assert call(n_seqs=1 << 27) == _lib.RSC_ERR_CAPACITY
+    assert call(n_seqs=1 << 40, max_drafts=1 << 40) == _lib.RSC_ERR_CAPACITY
+    torch.cuda.synchronize()
