@@ -523,6 +523,71 @@ RSC_API rsc_status rsc_verify_survivors(rsc_sampler *sampler, const rsc_draft_ba
                                         uint32_t *d_out_accepted, int32_t *d_out_status,
                                         void *stream);
 
+/*
+ * Distillation from a teacher's top tokens (no counterpart in the reference,
+ * which trains nothing): the loss of a student's logits against the
+ * log-probabilities that rsc_sample_ex lists for the teacher's rows
+ * (d_survivor_ids with d_survivor_logprobs), and its gradient. It trains the
+ * draft model whose tokens rsc_verify accepts.
+ *
+ * Row r has the student logits x (dtype, row_stride elements apart) and up to
+ * n[r] teacher entries (id_k, y_k). With v = x * (1/T), S = sum_j exp(v_j) and
+ * p_j = exp(v_j) / S:
+ *   tail == 0: t_k = exp(y_k) / sum_k exp(y_k), so y may be logits as well;
+ *              loss = sum_k t_k (log t_k - log p_k)
+ *   tail != 0: t_k = exp(y_k), y being log-probabilities over the whole
+ *              vocabulary; what is missing to 1, r = max(0, 1 - sum t), is
+ *              compared with the student's probability of all unlisted tokens:
+ *              loss = sum_k t_k (log t_k - log p_k)
+ *                     + r (log r - log(1 - sum_k p_k))
+ * y is taken as given: for a temperature the teacher's rows are sampled at that
+ * temperature (its log-probabilities are of the scaled logits). Entries with an
+ * id outside the vocabulary (the padding of the lists) or y = -inf are absent;
+ * an id listed twice counts twice in the loss and once in sum p. A row without
+ * an entry has loss 0 and no gradient. A student logit of -inf has p = 0 (a
+ * listed one gives loss +inf); a NaN or +inf logit, or a row of -inf alone,
+ * gives NaN, as a log-softmax does.
+ *
+ * Limits: cap <= RSC_DISTILL_MAX_TOP and rows <= 2^27 (RSC_ERR_CAPACITY), vocab
+ * <= 2^23 (RSC_ERR_VOCAB_TOO_LARGE). The handle gives the device; its capacity
+ * does not limit these calls, and they use none of its memory.
+ */
+#define RSC_DISTILL_MAX_TOP 1024
+typedef enum { RSC_F32 = 0, RSC_BF16 = 1, RSC_F16 = 2 } rsc_dtype;
+
+typedef struct rsc_distill_batch {
+    size_t rows;
+    size_t vocab;
+    const void *d_logits;     /* rows x vocab of dtype, aligned to its size             */
+    size_t row_stride;        /* elements between rows (>= vocab)                       */
+    int dtype;                /* rsc_dtype                                              */
+    int tail;
+    float temperature;        /* > 0, 1/T finite                                        */
+    size_t cap;               /* teacher slots per row                                  */
+    const uint32_t *d_n;      /* rows: entries of each row (above cap reads as cap); NULL: cap */
+    const uint32_t *d_ids;    /* rows x cap                                             */
+    const float *d_logprobs;  /* rows x cap                                             */
+} rsc_distill_batch;
+
+/*
+ * rsc_distill: the loss of every row (d_loss, f32) and, when d_dlogits is not
+ * NULL, in the same launch the gradient d(sum_r row_grads[r] * loss[r]) /
+ * d(logits) in the logits' type, rows grad_stride elements apart. A row with
+ * row_grads[r] == 0 gets a gradient of 0. d_dlogits may be d_logits itself
+ * (then grad_stride == row_stride): the gradient replaces the logits. d_state
+ * (rows x 4 f32, 16-byte aligned, nullable) keeps what rsc_distill_backward
+ * needs of a row.
+ *
+ * rsc_distill_backward: the gradient alone, from the same batch and the state of an
+ * earlier rsc_distill.
+ */
+RSC_API rsc_status rsc_distill(rsc_sampler *sampler, const rsc_distill_batch *batch, float *d_loss,
+                               float *d_state, const float *d_row_grads, void *d_dlogits,
+                               size_t grad_stride, void *stream);
+RSC_API rsc_status rsc_distill_backward(rsc_sampler *sampler, const rsc_distill_batch *batch,
+                                        const float *d_state, const float *d_row_grads,
+                                        void *d_dlogits, size_t grad_stride, void *stream);
+
 /* Number of kernel launches the library issued since the handle was created
  * (for the benchmark's launch count). */
 RSC_API uint64_t rsc_launch_count(const rsc_sampler *sampler);

@@ -83,6 +83,23 @@ pub(crate) struct RscSurvivorRecords {
     pub(crate) cap: usize,
 }
 
+/// `rsc_distill_batch`: student logits and the teacher's top tokens of each row.
+#[repr(C)]
+#[derive(Debug, Clone, Copy)]
+pub(crate) struct RscDistillBatch {
+    pub(crate) rows: usize,
+    pub(crate) vocab: usize,
+    pub(crate) d_logits: *const c_void,
+    pub(crate) row_stride: usize,
+    pub(crate) dtype: c_int,
+    pub(crate) tail: c_int,
+    pub(crate) temperature: f32,
+    pub(crate) cap: usize,
+    pub(crate) d_n: *const u32,
+    pub(crate) d_ids: *const u32,
+    pub(crate) d_logprobs: *const f32,
+}
+
 /// Opaque `rsc_sampler`.
 #[repr(C)]
 pub(crate) struct RscSampler {
@@ -348,6 +365,25 @@ unsafe extern "C" {
         d_out_tokens: *mut u32,
         d_out_accepted: *mut u32,
         d_out_status: *mut i32,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub(crate) fn rsc_distill(
+        sampler: *mut RscSampler,
+        batch: *const RscDistillBatch,
+        d_loss: *mut f32,
+        d_state: *mut f32,
+        d_row_grads: *const f32,
+        d_dlogits: *mut c_void,
+        grad_stride: usize,
+        stream: *mut c_void,
+    ) -> c_int;
+    pub(crate) fn rsc_distill_backward(
+        sampler: *mut RscSampler,
+        batch: *const RscDistillBatch,
+        d_state: *const f32,
+        d_row_grads: *const f32,
+        d_dlogits: *mut c_void,
+        grad_stride: usize,
         stream: *mut c_void,
     ) -> c_int;
     pub(crate) fn rsc_launch_count(sampler: *const RscSampler) -> u64;

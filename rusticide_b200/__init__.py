@@ -5,6 +5,7 @@ package is its Python host side: the ctypes binding, a mirror of the
 reference's Sampler API, and the synthetic logit generator of the benchmark.
 """
 
+from .distill import distill_loss  # noqa: F401
 from .sampler import (  # noqa: F401
     Engine,
     InvalidShape,
@@ -21,5 +22,5 @@ from .sampler import (  # noqa: F401
 
 __all__ = [
     "Engine", "InvalidShape", "NoValidTokens", "Sampler", "SamplingError", "SamplingParams",
-    "TensorError", "VocabOverflow", "engine", "extract_logits", "row_error",
+    "TensorError", "VocabOverflow", "distill_loss", "engine", "extract_logits", "row_error",
 ]

@@ -31,6 +31,8 @@ RSC_ROW_FLAG_DRAW_NEAR_BOUNDARY = 1 << 8
 RSC_ROW_FLAG_LARGE_PATH = 1 << 9
 
 RSC_SHARD_TIE_CAP = 24
+RSC_DISTILL_MAX_TOP = 1024
+RSC_F32, RSC_BF16, RSC_F16 = 0, 1, 2  # rsc_dtype
 RSC_NOALLOC_SCRATCH_BYTES = 64 << 20
 RSC_NOALLOC_MAX_VOCAB = RSC_NOALLOC_SCRATCH_BYTES // 16
 
@@ -105,6 +107,24 @@ class RscSurvivorRecords(ctypes.Structure):
     ]
 
 
+class RscDistillBatch(ctypes.Structure):
+    """rsc_distill_batch: student logits and the teacher's top tokens of each row."""
+
+    _fields_ = [
+        ("rows", ctypes.c_size_t),
+        ("vocab", ctypes.c_size_t),
+        ("d_logits", ctypes.c_void_p),
+        ("row_stride", ctypes.c_size_t),
+        ("dtype", ctypes.c_int),
+        ("tail", ctypes.c_int),
+        ("temperature", ctypes.c_float),
+        ("cap", ctypes.c_size_t),
+        ("d_n", ctypes.c_void_p),
+        ("d_ids", ctypes.c_void_p),
+        ("d_logprobs", ctypes.c_void_p),
+    ]
+
+
 # Every symbol the header declares, with its ctypes signature.
 _P = ctypes.c_void_p
 _SZ = ctypes.c_size_t
@@ -146,6 +166,8 @@ SIGNATURES = {
     "rsc_verify_survivors": (_ST, [_P, ctypes.POINTER(RscDraftBatch),
                                    ctypes.POINTER(RscSurvivorRecords),
                                    ctypes.POINTER(RscSurvivorRecords), _P, _P, _P, _P, _P, _P]),
+    "rsc_distill": (_ST, [_P, ctypes.POINTER(RscDistillBatch), _P, _P, _P, _P, _SZ, _P]),
+    "rsc_distill_backward": (_ST, [_P, ctypes.POINTER(RscDistillBatch), _P, _P, _P, _SZ, _P]),
     "rsc_launch_count": (ctypes.c_uint64, [_P]),
     "rsc_debug_hold_scratch": (_ST, [_P, ctypes.c_int, _P]),
 }

@@ -856,6 +856,77 @@ rsc_status rsc_verify_survivors(rsc_sampler *s, const rsc_draft_batch *x,
     return cuda_status(rsc::launch_verify_records(c, static_cast<cudaStream_t>(stream)));
 }
 
+namespace {
+
+rsc_status check_distill(const rsc_sampler *s, const rsc_distill_batch *x, const float *row_grads,
+                         const void *dlogits, size_t grad_stride, rsc::DistillCall &c) {
+    if (!s || !s->alive) return RSC_ERR_NOT_INITIALIZED;
+    if (!x) return RSC_ERR_INVALID_ARGUMENT;
+    if (x->vocab > rsc::kDistillMaxVocab) return RSC_ERR_VOCAB_TOO_LARGE;
+    if (x->rows > rsc::kDistillMaxRows || x->cap > rsc::kDistillMaxTop) return RSC_ERR_CAPACITY;
+    if (x->dtype != RSC_F32 && x->dtype != RSC_BF16 && x->dtype != RSC_F16)
+        return RSC_ERR_INVALID_ARGUMENT;
+    const float scale = 1.0f / x->temperature;
+    if (!(x->temperature > 0.0f) || !std::isfinite(scale) || !(scale > 0.0f))
+        return RSC_ERR_INVALID_ARGUMENT;
+    if (x->rows == 0) return RSC_OK;
+    if (x->vocab == 0) return RSC_ERR_INVALID_SHAPE;
+    const size_t size = x->dtype == RSC_F32 ? 4 : 2;
+    if (!x->d_logits || misaligned(x->d_logits, size)) return RSC_ERR_INVALID_ARGUMENT;
+    if (x->cap > 0 && (!x->d_ids || !x->d_logprobs)) return RSC_ERR_INVALID_ARGUMENT;
+    if (x->rows > 1 && x->row_stride < x->vocab) return RSC_ERR_INVALID_SHAPE;
+    if (dlogits) {
+        if (!row_grads || misaligned(dlogits, size)) return RSC_ERR_INVALID_ARGUMENT;
+        if (x->rows > 1 && (grad_stride < x->vocab ||
+                            (dlogits == x->d_logits && grad_stride != x->row_stride)))
+            return RSC_ERR_INVALID_SHAPE;
+    }
+    c.rows = static_cast<uint32_t>(x->rows);
+    c.vocab = static_cast<uint32_t>(x->vocab);
+    c.scale = scale;
+    c.tail = x->tail != 0;
+    c.logits = x->d_logits;
+    c.row_stride = x->row_stride;
+    c.cap = x->cap;
+    c.n = x->d_n;
+    c.ids = x->d_ids;
+    c.logprobs = x->d_logprobs;
+    c.row_grads = row_grads;
+    c.dlogits = const_cast<void *>(dlogits);
+    c.grad_stride = grad_stride;
+    return RSC_OK;
+}
+
+}  // namespace
+
+rsc_status rsc_distill(rsc_sampler *s, const rsc_distill_batch *x, float *d_loss, float *d_state,
+                       const float *d_row_grads, void *d_dlogits, size_t grad_stride, void *stream) {
+    rsc::DistillCall c{};
+    rsc_status st = check_distill(s, x, d_row_grads, d_dlogits, grad_stride, c);
+    if (st != RSC_OK || x->rows == 0) return st;
+    if (!d_loss || misaligned(d_state, 16)) return RSC_ERR_INVALID_ARGUMENT;
+    c.loss = d_loss;
+    c.state = d_state;
+    DeviceGuard guard(s->device);
+    ++s->launches;
+    return cuda_status(rsc::launch_distill(c, static_cast<rsc_dtype>(x->dtype), true, d_dlogits != nullptr,
+                                           s->num_sms, static_cast<cudaStream_t>(stream)));
+}
+
+rsc_status rsc_distill_backward(rsc_sampler *s, const rsc_distill_batch *x, const float *d_state,
+                                const float *d_row_grads, void *d_dlogits, size_t grad_stride,
+                                void *stream) {
+    rsc::DistillCall c{};
+    rsc_status st = check_distill(s, x, d_row_grads, d_dlogits, grad_stride, c);
+    if (st != RSC_OK || x->rows == 0) return st;
+    if (!d_dlogits || !d_state || misaligned(d_state, 16)) return RSC_ERR_INVALID_ARGUMENT;
+    c.state = const_cast<float *>(d_state);
+    DeviceGuard guard(s->device);
+    ++s->launches;
+    return cuda_status(rsc::launch_distill(c, static_cast<rsc_dtype>(x->dtype), false, true, s->num_sms,
+                                           static_cast<cudaStream_t>(stream)));
+}
+
 uint64_t rsc_launch_count(const rsc_sampler *s) { return s && s->alive ? s->launches : 0; }
 
 rsc_status rsc_debug_hold_scratch(rsc_sampler *s, int hold, void *stream) {

@@ -244,6 +244,32 @@ cudaError_t launch_verify(const VerifyCall &c, bool greedy, int num_sms, uint64_
                           cudaStream_t stream);
 cudaError_t launch_verify_records(const VerifyCall &c, cudaStream_t stream);
 
+// Distillation from a teacher's top tokens (distill.cu).
+constexpr uint32_t kDistillMaxTop = RSC_DISTILL_MAX_TOP;
+constexpr uint64_t kDistillMaxVocab = uint64_t{1} << 23;
+constexpr uint64_t kDistillMaxRows = uint64_t{1} << 27;
+
+struct DistillCall {
+    uint32_t rows, vocab;
+    float scale;
+    int tail;
+    const void *logits;
+    size_t row_stride;
+    size_t cap;             // teacher slots per row, at most kDistillMaxTop
+    const uint32_t *n;      // [rows], nullable
+    const uint32_t *ids;    // [rows][cap]
+    const float *logprobs;  // [rows][cap]
+    const float *row_grads; // [rows] (gradient only)
+    void *dlogits;          // gradient, row r at dlogits + r * grad_stride elements
+    size_t grad_stride;
+    float *loss;            // [rows] (forward only)
+    float *state;           // [rows][4]: maximum, 1 / sum, unlisted maximum, unlisted factor; nullable in forward
+};
+
+// One launch: the loss (forward), its gradient, or both. rows, vocab > 0.
+cudaError_t launch_distill(const DistillCall &c, rsc_dtype dtype, bool forward, bool grad, int num_sms,
+                           cudaStream_t stream);
+
 // Shared-memory bytes of the streaming kernel (for occupancy queries).
 size_t stream_topk_smem_bytes();
 

@@ -1,0 +1,47 @@
+"""Training a draft model on the tokens its target model prefers.
+
+`distill_loss` is the differentiable form of the engine's distillation call: the teacher's rows are
+given as the survivors and log-probabilities that `Engine.sample_ex(..., logprobs=True)` lists for
+them, the student's as logits. Drafts of a student trained this way are what `Engine.verify` accepts
+more of. The reference (crates/rusticide-model) serves models and trains none; nothing there
+corresponds to this module.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from .sampler import engine
+
+
+class _DistillLoss(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, ids, logprobs, n, temperature, tail):
+        want = ctx.needs_input_grad[0]
+        loss, state = engine(logits.device).distill_forward(
+            logits, ids, logprobs, n, temperature, tail, want_state=want)
+        if want:
+            ctx.save_for_backward(logits, ids, logprobs, n, state)
+            ctx.how = (temperature, tail)
+        return loss
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad_loss):
+        logits, ids, logprobs, n, state = ctx.saved_tensors
+        grad = engine(logits.device).distill_backward(
+            logits, ids, logprobs, state, grad_loss.contiguous(), n, *ctx.how)
+        return grad, None, None, None, None, None
+
+
+def distill_loss(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor,
+                 n: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                 tail: bool = False) -> torch.Tensor:
+    """Loss of every row of student logits [..., vocab] against a teacher's top tokens ids
+    [..., top] int32 with log-probabilities logprobs [..., top] f32 (see rsc_distill in the C
+    header), n [...] int32 of them a row. Returns [...] f32; differentiable once, with respect to
+    the logits. A training loop that knows each row's weight beforehand takes
+    `Engine.distill_step`, which gives loss and gradient in one pass."""
+    return _DistillLoss.apply(logits, ids, logprobs, n, float(temperature), bool(tail))

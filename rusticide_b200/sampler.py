@@ -114,6 +114,9 @@ def _stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
+_DISTILL_TYPES = {torch.float32: _lib.RSC_F32, torch.bfloat16: _lib.RSC_BF16, torch.float16: _lib.RSC_F16}
+
+
 # ---------------------------------------------------------------------------
 # Engine: one rsc_sampler handle per device, grown on demand.
 # ---------------------------------------------------------------------------
@@ -549,6 +552,88 @@ class Engine:
                                             status.data_ptr(), _stream_ptr(self.device)),
               "rsc_verify_survivors")
         return tokens, accepted, status
+
+    # -- distillation from a teacher's top tokens ------------------------------
+    def _distill_batch(self, logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor,
+                       n: Optional[torch.Tensor], temperature: float, tail: bool):
+        """The C batch of [..., vocab] logits and [..., top] teacher entries, with the tensors it
+        points into (kept until the call has been issued)."""
+        if logits.device != self.device:
+            raise ValueError(f"logits on {logits.device}, engine on {self.device}")
+        dtype = _DISTILL_TYPES.get(logits.dtype)
+        if dtype is None:
+            raise TensorError("f32, bf16 or f16", str(logits.dtype).replace("torch.", ""))
+        if logits.dim() < 1 or ids.shape[:-1] != logits.shape[:-1] or ids.dim() != logits.dim():
+            raise InvalidShape(list(ids.shape))
+        lead, vocab, cap = logits.shape[:-1], logits.shape[-1], ids.shape[-1]
+        rows = 1
+        for k in lead:
+            rows *= k
+        x = logits if logits.dim() == 2 else logits.reshape(rows, vocab)
+        if rows > 0 and vocab > 1 and (x.stride(1) != 1 or (rows > 1 and x.stride(0) < vocab)):
+            x = x.contiguous()  # rows out of order, or one row broadcast to many
+        b = _lib.RscDistillBatch()
+        b.rows, b.vocab, b.dtype, b.tail, b.temperature, b.cap = (
+            rows, vocab, dtype, bool(tail), float(temperature), cap)
+        b.d_logits, b.row_stride = x.data_ptr(), x.stride(0) if rows > 1 else vocab
+        b.d_ids = self._want(ids, "ids", torch.int32, (*lead, cap))
+        b.d_logprobs = self._want(logprobs, "logprobs", torch.float32, (*lead, cap))
+        if n is not None:
+            b.d_n = self._want(n, "n", torch.int32, lead)
+        return b, x
+
+    def distill_forward(self, logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor,
+                        n: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                        tail: bool = False, want_state: bool = True):
+        """rsc_distill without a gradient. Returns (loss [...] f32, state): the loss of every row of
+        `logits` [..., vocab] (f32, bf16 or f16) against the teacher's entries ids [..., top] int32
+        and logprobs [..., top] f32, n [...] int32 of them (None: all; ids of -1 are skipped), and
+        the state that distill_backward takes (None without want_state)."""
+        b, x = self._distill_batch(logits, ids, logprobs, n, temperature, tail)
+        loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=self.device)
+        state = torch.empty((b.rows, 4), dtype=torch.float32, device=self.device) if want_state else None
+        check(self.lib.rsc_distill(self._h, ctypes.byref(b), loss.data_ptr(), _ptr(state), None, None,
+                                   0, _stream_ptr(self.device)), "rsc_distill")
+        return loss, state
+
+    def distill_step(self, logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor,
+                     row_grads: torch.Tensor, n: Optional[torch.Tensor] = None,
+                     temperature: float = 1.0, tail: bool = False,
+                     out: Optional[torch.Tensor] = None):
+        """rsc_distill with its gradient in the same pass: (loss [...], d(sum row_grads * loss) /
+        d logits in the logits' type). row_grads [...] f32 is what each row's loss counts (its
+        weight over the batch size, 0 for padding). `out` takes the gradient; it may be `logits`
+        itself, which the gradient then replaces."""
+        b, x = self._distill_batch(logits, ids, logprobs, n, temperature, tail)
+        up = self._want(row_grads, "row_grads", torch.float32, logits.shape[:-1])
+        if out is None:
+            out = torch.empty(logits.shape, dtype=logits.dtype, device=self.device)
+            stride = b.vocab
+        else:
+            if out is not logits:
+                stride = b.vocab
+                self._want(out, "out", logits.dtype, logits.shape)
+            elif x.data_ptr() != logits.data_ptr():
+                raise ValueError("logits of this layout cannot be replaced by their gradient")
+            else:
+                stride = b.row_stride
+        loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=self.device)
+        check(self.lib.rsc_distill(self._h, ctypes.byref(b), loss.data_ptr(), None, up, out.data_ptr(),
+                                   stride, _stream_ptr(self.device)), "rsc_distill")
+        return loss, out
+
+    def distill_backward(self, logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor,
+                         state: torch.Tensor, row_grads: torch.Tensor,
+                         n: Optional[torch.Tensor] = None, temperature: float = 1.0,
+                         tail: bool = False) -> torch.Tensor:
+        """rsc_distill_backward: the gradient from an earlier distill_forward's state."""
+        b, x = self._distill_batch(logits, ids, logprobs, n, temperature, tail)
+        up = self._want(row_grads, "row_grads", torch.float32, logits.shape[:-1])
+        st = self._want(state, "state", torch.float32, (b.rows, 4))
+        grad = torch.empty(logits.shape, dtype=logits.dtype, device=self.device)
+        check(self.lib.rsc_distill_backward(self._h, ctypes.byref(b), st, up, grad.data_ptr(), b.vocab,
+                                            _stream_ptr(self.device)), "rsc_distill_backward")
+        return grad
 
     # -- LM head with the sampler fused into its epilogue ----------------------
     @staticmethod
