@@ -110,21 +110,16 @@ __device__ __forceinline__ void sum_join(float &m, double &s, float m2, double s
     }
 }
 
+// The sums of `width` neighbouring lanes joined, in every one of them: the
+// maximum first, then each lane's sum brought to it by one exponential (whose
+// error, as a batch's, is within 4e-6).
 __device__ __forceinline__ void sum_join_lanes(float &m, double &s, int width) {
-    for (int o = width / 2; o > 0; o >>= 1) {
-        const float m2 = __shfl_xor_sync(0xffffffffu, m, o, width);
-        const double s2 = __shfl_xor_sync(0xffffffffu, s, o, width);
-        // Both lanes of a pair join in the same order, so they agree.
-        if ((threadIdx.x & o) == 0) {
-            sum_join(m, s, m2, s2);
-        } else {
-            float mm = m2;
-            double ss = s2;
-            sum_join(mm, ss, m, s);
-            m = mm;
-            s = ss;
-        }
-    }
+    float top = m;
+    for (int o = width / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    // A lane at -inf holds 0 or NaN, which stays.
+    if (m != kNegInf) s *= static_cast<double>(exp_fast(__fsub_rn(m, top)));
+    for (int o = width / 2; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    m = top;
 }
 
 }  // namespace rsc

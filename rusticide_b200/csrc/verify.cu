@@ -24,6 +24,8 @@
 //     those sums where their error bound allows it, sums the first undecided
 //     or refused position's rows once more in binary64, decides it exactly, and
 //     draws the last token from binary64 running sums.
+#include <algorithm>
+
 #include <cooperative_groups.h>
 
 #include "rsc_common.cuh"
@@ -39,7 +41,7 @@ namespace {
 constexpr int kRowThreads = 256;
 constexpr int kDrawThreads = 256;
 constexpr int kDrawWarps = kDrawThreads / 32;
-constexpr uint32_t kDrawMaxCtas = 8;  // the largest portable cluster
+constexpr uint32_t kDrawMaxCtas = 16;  // the largest cluster (8 is the largest portable one)
 
 // Part of a row, as the first launch leaves it: (maximum, sum of exp(v -
 // maximum)), or for greedy calls the packed (total-order key, index) of the
@@ -279,23 +281,51 @@ verify_greedy_kernel(const __grid_constant__ VerifyCall c) {
 // Launch 2: decisions and the last token.
 // ---------------------------------------------------------------------------
 
-// exp(d) in binary64 for d <= 0: d = k ln2 / 256 + r with |r| <= ln2 / 512,
-// exp(d) = 2^(k/256) * (1 + r + r^2/2 + r^3/6 + r^4/24). The first neglected
-// term, r^5/120, is below 4e-17. `tab` holds 2^(j/256). Below -700 the result
-// is 0: no such term changes a sum whose largest is 1.
-__device__ __forceinline__ double exp64(double d, const double *tab) {
-    constexpr double kMagic = 0x1.8p+52;
-    if (!(d > -700.0)) return 0.0;
-    const double k0 = __fma_rn(d, 256.0 * 1.4426950408889634074, kMagic);
-    const int32_t k = __double2loint(k0);
-    const double kd = __dsub_rn(k0, kMagic);
-    const double r = __fma_rn(kd, -0.69314718055994530942 / 256.0, d);
-    double p = __fma_rn(r, 1.0 / 24.0, 1.0 / 6.0);
-    p = __fma_rn(p, r, 0.5);
-    p = __fma_rn(p, r, 1.0);
-    const double t = tab[k & 255];
-    const double scaled = __hiloint2double(__double2hiint(t) + ((k >> 8) << 20), __double2loint(t));
-    return __fma_rn(scaled, __dmul_rn(p, r), scaled);
+// What exp(v - max) of a row is taken with. Terms that far below the maximum
+// (-inf and NaN among them) that exp would leave binary64 are held at exp(-700),
+// 1e-304, so that no term needs a branch: no sum that counts feels it. Weights
+// up to kNoWeight are those of such terms.
+struct RowBase {
+    float scale, max32;
+    double max;
+    __device__ __forceinline__ RowBase() {}
+    __device__ __forceinline__ RowBase(float scale_, float max_) : scale(scale_), max32(max_), max(max_) {}
+};
+constexpr double kNoWeight = 1e-280;
+
+constexpr uint32_t kExpSteps = 512;  // entries of the table 2^(j / kExpSteps)
+
+// exp(v - max) in binary64, v = x * scale. With d = v - max = k ln2 / 512 + r
+// it is 2^(k/512) * (1 + r + r^2/2 + r^3/6); k comes from d in binary32, which
+// leaves |r| below 0.6 ln2 / 512 = 8.2e-4, and the first neglected term, r^4/24,
+// below 2e-14. What bounds a pass is the chain of dependent binary64 operations
+// (and their rate, 16 lanes a cycle and scheduler), so k does not wait for
+// them and the polynomial is two deep. d <= 0 apart from a row summed against
+// its first block; negative ones order by magnitude in their high words, so
+// the nearer of d and -700 is an integer minimum (positive ones pass it).
+__device__ __forceinline__ double exp64(float x, const RowBase &b, const double *tab) {
+    const float v = masked_scaled(x, b.scale);
+    const double far = __dsub_rn(static_cast<double>(v), b.max);
+    const uint32_t high = min(static_cast<uint32_t>(__double2hiint(far)), 0xc085e000u);  // -700
+    const double d = __hiloint2double(static_cast<int>(high), __double2loint(far));
+    const float kf = __fmaf_rn(fmaxf(__fsub_rn(v, b.max32), -700.0f), kExpSteps * 1.44269504f, 0x1.8p+23f);
+    const uint32_t k = __float_as_uint(kf) - 0x4b400000u;
+    // 2^52 + 2^31 + k, less 2^52 + 2^31.
+    const double kd = __dsub_rn(__hiloint2double(0x43300000, static_cast<int>(k ^ 0x80000000u)),
+                                0x1p+52 + 0x1p+31);
+    const double r = __fma_rn(kd, -0.69314718055994530942 / kExpSteps, d);
+    const double p = __fma_rn(__dmul_rn(r, r), __fma_rn(r, 1.0 / 6.0, 0.5), r);
+    const double t = tab[k % kExpSteps];
+    const double scaled = __hiloint2double(
+        __double2hiint(t) + static_cast<int>((k & ~(kExpSteps - 1u)) << 11), __double2loint(t));
+    return __fma_rn(scaled, p, scaled);
+}
+static_assert(kExpSteps == 512, "k / 512 goes to bit 20 of the high word");
+
+// The same with the floor's terms as the zeros they stand for.
+__device__ __forceinline__ double exp64_or_zero(float x, const RowBase &b, const double *tab) {
+    const double e = exp64(x, b, tab);
+    return e > kNoWeight ? e : 0.0;
 }
 
 enum Weight : int {
@@ -304,40 +334,63 @@ enum Weight : int {
     kWeightResidual = 2,  // max(p - q, 0)
 };
 
-// What a draw sums over: v of the target row against its maximum, and for the
-// residual the draft row's and both reciprocal sums.
+// The weights a draw runs over: P = exp(v - max) of the target row, or P -
+// kappa Q with Q the same of the draft row and kappa = sum P / sum Q.
 struct Draw {
     const float *p;
     const float *q;
-    double max_p, max_q;
-    double inv_p, inv_q;
+    RowBase base_p, base_q;
+    double kappa;
     uint32_t without;
     int weight;
 };
 
+__device__ __forceinline__ double weight_of(const Draw &d, uint32_t j, float x, float y,
+                                            const double *tab) {
+    const double e = exp64(x, d.base_p, tab);
+    if (d.weight == kWeightResidual) return fmax(e - d.kappa * exp64(y, d.base_q, tab), 0.0);
+    return d.weight == kWeightWithout && j == d.without ? 0.0 : e;
+}
+
+// The residual in one pass. Its weights need kappa, the quotient of the very
+// sums that the pass makes; what is there beforehand is the binary32 sums'
+// quotient, within 1.5e-5 of it. That settles for nearly every token whether
+// P > kappa Q, so the pass adds up, over the tokens above it, D = P - kappa~ Q
+// and Q, and their weight is D + (kappa~ - kappa) Q once kappa is known. The few
+// tokens with |P - kappa~ Q| below 2^-16 of kappa~ Q (four of 151936, where the
+// rows differ by a normal of width 1/2) are kept apart. A cluster that finds
+// more of them than it keeps, as where the rows are equal, sums the weights in
+// a second pass.
+constexpr uint32_t kNearWarp = 4;  // kept by a warp
+constexpr uint32_t kNearCta = 16;  // and by its CTA
+
+// A CTA's sums, as the cluster sees them.
+struct CtaSums {
+    // Row: sum, reference, maximum. Without: sum, sum without the token.
+    // Residual: sum of P, of Q, of D, of Q where D counts. Weights: the sum.
+    double s[4];
+    uint32_t n_near;  // above kNearCta: too many
+    double near[kNearCta][2];
+};
+
 struct DrawShared {
-    double tab[256];
-    double warp_sum[kDrawWarps][2];
+    double tab[kExpSteps];
+    double warp_sum[kDrawWarps][4];
+    double warp_near[kDrawWarps][kNearWarp][2];
+    uint32_t warp_n_near[kDrawWarps];
+    double cta_near[kNearCta][2];
+    double warp_weight[kDrawWarps];
     // Two sets, used in turn: a CTA may write the next sums while a peer still
     // reads the last ones.
-    double cta_sum[2][kDrawMaxCtas][2];
-    float warp_max[kDrawWarps];
-    float cta_max[kDrawMaxCtas];
+    CtaSums cta[2][kDrawMaxCtas];
     // The position at hand, decided by every CTA of the cluster alike.
     uint32_t first;
     float max_p[kDrawWarps], max_q[kDrawWarps];
-    float pos_max_p, pos_max_q;
+    double kappa[kDrawWarps];
+    // What each warp's position was tested with: u, and both rows' logits of the token.
+    float test_u[kDrawWarps], test_p[kDrawWarps], test_q[kDrawWarps];
+    uint32_t test_token[kDrawWarps];
 };
-
-__device__ __forceinline__ double weight_at(const Draw &d, uint32_t j, float scale,
-                                            const double *tab) {
-    const double e = exp64(static_cast<double>(masked_scaled(d.p[j], scale)) - d.max_p, tab);
-    if (d.weight == kWeightResidual) {
-        const double f = exp64(static_cast<double>(masked_scaled(d.q[j], scale)) - d.max_q, tab);
-        return fmax(e * d.inv_p - f * d.inv_q, 0.0);
-    }
-    return d.weight == kWeightWithout && j == d.without ? 0.0 : e;
-}
 
 // [lo, hi) cut into kDrawWarps runs whose length is a multiple of 32.
 __device__ __forceinline__ void warp_run(uint32_t lo, uint32_t hi, uint32_t w, uint32_t &wlo,
@@ -347,75 +400,192 @@ __device__ __forceinline__ void warp_run(uint32_t lo, uint32_t hi, uint32_t w, u
     whi = min(hi, wlo + len);
 }
 
-// This warp's sum of the weights over its run of [lo, hi) into warp_sum[w][0].
-__device__ __forceinline__ double run_sum(const Draw &d, uint32_t wlo, uint32_t whi, float scale,
+// Calls f(first index, target logits, draft logits) for the blocks of 32 *
+// kLoads elements of a warp's run, lane l holding elements first + 32 k + l
+// (single words: the two rows need not share an alignment). Behind the run's
+// end the logits read -inf.
+template <bool kPair, int kLoads, typename F>
+__device__ __forceinline__ void visit_run(const float *p, const float *q, uint32_t wlo, uint32_t whi,
+                                          F f) {
+    const uint32_t lane = threadIdx.x & 31u;
+    uint32_t j0 = wlo;
+    float x[kLoads], y[kLoads];
+#pragma unroll 1
+    for (; j0 + 32 * kLoads <= whi; j0 += 32 * kLoads) {
+        const float *pj = p + j0 + lane;
+        const float *qj = q + j0 + lane;
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k) {
+            x[k] = __ldg(pj + 32 * k);
+            y[k] = kPair ? __ldg(qj + 32 * k) : kNegInf;
+        }
+        f(j0, x, y);
+    }
+    if (j0 < whi) {
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k) {
+            const uint32_t j = j0 + 32 * k + lane;
+            x[k] = j < whi ? __ldg(p + j) : kNegInf;
+            y[k] = kPair && j < whi ? __ldg(q + j) : kNegInf;
+        }
+        f(j0, x, y);
+    }
+}
+constexpr int kRowLoads = 16;  // sixteen exponentials at a time
+constexpr int kPairLoads = 8;  // likewise
+
+// This warp's sum of the weights over its run.
+__device__ __forceinline__ double run_sum(const Draw &d, uint32_t wlo, uint32_t whi,
                                           const double *tab) {
     double s = 0.0;
-    for (uint32_t j = wlo + (threadIdx.x & 31u); j < whi; j += 32) s += weight_at(d, j, scale, tab);
+    auto add = [&](uint32_t j0, const float *x, const float *y) {
+#pragma unroll
+        for (int k = 0; k < kPairLoads; ++k)
+            s += weight_of(d, j0 + 32 * k + (threadIdx.x & 31u), x[k], y[k], tab);
+    };
+    if (d.weight == kWeightResidual)
+        visit_run<true, kPairLoads>(d.p, d.q, wlo, whi, add);
+    else
+        visit_run<false, kPairLoads>(d.p, d.q, wlo, whi, add);
     return warp_sum(s);
 }
 
-__global__ void __launch_bounds__(kDrawThreads)
+// Inclusive sums over the lanes.
+__device__ __forceinline__ double warp_scan(double s) {
+    const uint32_t lane = threadIdx.x & 31u;
+#pragma unroll
+    for (int o = 1; o < 32; o *= 2) {
+        const double up = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= static_cast<uint32_t>(o)) s += up;
+    }
+    return s;
+}
+
+// Of the lanes' sums of weights, the first whose running total exceeds `rest`;
+// `rest` becomes what is wanted within it. Where rounding leaves none, the last
+// lane of any weight, with all of it wanted. The same in every lane.
+__device__ __forceinline__ uint32_t locate(double s, double &rest) {
+    const bool some = s > kNoWeight;
+    const double upto = warp_scan(s);
+    const uint32_t hit = __ballot_sync(0xffffffffu, some && upto > rest);
+    const uint32_t any = __ballot_sync(0xffffffffu, some);
+    if (hit == 0) {
+        rest = __longlong_as_double(0x7ff0000000000000ll);
+        return any ? 31u - __clz(any) : 0u;
+    }
+    const uint32_t at = __ffs(hit) - 1u;
+    const double before = __shfl_sync(0xffffffffu, upto, at ? at - 1u : 0u);
+    if (at) rest -= before;
+    return at;
+}
+
+// The weight of a run or a CTA from its residual sums, kappa known.
+__device__ __forceinline__ double residual_weight(double sum_d, double sum_q, double slip,
+                                                  double kappa, const double (*near)[2],
+                                                  uint32_t n_near) {
+    double s = sum_d + slip * sum_q;
+    for (uint32_t k = 0; k < n_near; ++k) s += fmax(near[k][0] - kappa * near[k][1], 0.0);
+    return s;
+}
+
+__global__ void __launch_bounds__(kDrawThreads, 2)
 verify_draw_kernel(const __grid_constant__ VerifyCall c, uint32_t ctas) {
-    __shared__ DrawShared sh;
+    extern __shared__ __align__(16) unsigned char draw_smem[];
+    DrawShared &sh = *reinterpret_cast<DrawShared *>(draw_smem);
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t rank = cluster.block_rank();
     const uint32_t b = blockIdx.x / ctas;
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    for (uint32_t j = threadIdx.x; j < 256; j += kDrawThreads) sh.tab[j] = exp2(j / 256.0);
+    for (uint32_t j = threadIdx.x; j < kExpSteps; j += kDrawThreads)
+        sh.tab[j] = exp2(static_cast<double>(j) / kExpSteps);
     const uint32_t n = drafts_of(c, b);
     const uint32_t *drafts = c.draft_tokens + static_cast<size_t>(b) * c.max_drafts;
     const uint32_t seg = ((c.vocab + ctas - 1) / ctas + 31u) & ~31u;
     const uint32_t lo = min(c.vocab, rank * seg), hi = min(c.vocab, lo + seg);
     uint32_t wlo, whi;
     warp_run(lo, hi, warp, wlo, whi);
-    // A CTA's partial sums to every CTA of the cluster, and their total in
-    // rank order.
-    uint32_t set = 1;
-    auto share_sums = [&](double a0, double a1, double &t0, double &t1) {
-        set ^= 1u;
-        __syncthreads();
-        if (lane == 0) {
-            sh.warp_sum[warp][0] = a0;
-            sh.warp_sum[warp][1] = a1;
-        }
-        __syncthreads();
-        if (threadIdx.x < ctas) {
-            double s0 = 0.0, s1 = 0.0;
-            for (int w = 0; w < kDrawWarps; ++w) {
-                s0 += sh.warp_sum[w][0];
-                s1 += sh.warp_sum[w][1];
-            }
-            double *to = &cluster.map_shared_rank(&sh, threadIdx.x)->cta_sum[set][rank][0];
-            to[0] = s0;
-            to[1] = s1;
-        }
-        cluster.sync();
-        t0 = t1 = 0.0;
-        for (uint32_t r = 0; r < ctas; ++r) {
-            t0 += sh.cta_sum[set][r][0];
-            t1 += sh.cta_sum[set][r][1];
-        }
+    // What a test needs besides the row sums, fetched while those are still
+    // being made. A warp looks at one position, lanes 0-15 at its target row,
+    // lanes 16-31 at its draft row.
+    const bool drafted = lane >= 16;
+    auto fetch = [&](uint32_t i, uint32_t &t, float &u, float &x) {
+        t = drafts[i];
+        u = uniform_of(c, b, i, false);
+        x = kNegInf;
+        if (t < c.vocab && (c.draft || !drafted))
+            x = (drafted ? draft_row(c, b, i) : target_row(c, b, i))[t];
     };
+    uint32_t test_token = 0;
+    float test_u = 0.0f, test_x = 0.0f;
+    if (warp < n) fetch(warp, test_token, test_u, test_x);
+    const float last_u = c.uniforms ? uniform_of(c, b, 0, true) : 0.0f;
     cluster.sync();  // every CTA of the cluster runs before its memory is written
     asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    uint32_t set = 1;  // the set of sums in use
+    // The CTA's sums (this warp's, every lane alike) to the whole cluster.
+    auto share = [&](double s0, double s1, double s2, double s3, uint32_t n_near) {
+        set ^= 1u;
+        if (lane == 0) {
+            sh.warp_sum[warp][0] = s0;
+            sh.warp_sum[warp][1] = s1;
+            sh.warp_sum[warp][2] = s2;
+            sh.warp_sum[warp][3] = s3;
+            sh.warp_n_near[warp] = n_near;
+        }
+        __syncthreads();
+        if (warp == 0) {
+            const bool in = lane < kDrawWarps;
+            double s[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s[k] = warp_sum(in ? sh.warp_sum[lane][k] : 0.0);
+            // The kept tokens in the order of the warps.
+            const uint32_t mine = in ? sh.warp_n_near[lane] : 0u;
+            uint32_t upto = min(mine, kNearWarp);
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const uint32_t up = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= static_cast<uint32_t>(o)) upto += up;
+            }
+            uint32_t count = __shfl_sync(0xffffffffu, upto, 31);
+            if (__any_sync(0xffffffffu, mine > kNearWarp) || count > kNearCta) count = kNearCta + 1u;
+            if (count <= kNearCta)
+                for (uint32_t k = 0; k < min(mine, kNearWarp); ++k) {
+                    sh.cta_near[upto - mine + k][0] = sh.warp_near[lane][k][0];
+                    sh.cta_near[upto - mine + k][1] = sh.warp_near[lane][k][1];
+                }
+            __syncwarp();
+            if (lane < ctas) {
+                CtaSums &to = cluster.map_shared_rank(&sh, lane)->cta[set][rank];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) to.s[k] = s[k];
+                to.n_near = count;
+                for (uint32_t k = 0; count <= kNearCta && k < count; ++k) {
+                    to.near[k][0] = sh.cta_near[k][0];
+                    to.near[k][1] = sh.cta_near[k][1];
+                }
+            }
+        }
+        cluster.sync();
+    };
+    auto cta_sum = [&](int k) { return lane < ctas ? sh.cta[set][lane].s[k] : 0.0; };
 
     uint32_t a = 0;
     int32_t status = RSC_ROW_OK;
     Draw d{};
-    // The weights' sums are left in warp_sum[.][1] and cta_sum[set][.][1].
-    double total = 0.0;
+    // Filled once the last token's row is settled: the weight of lane r's CTA and
+    // their sum, and the weights of this CTA's runs (warp_weight) on its own scale.
+    double cta_weight = 0.0, total = 0.0, own_scale = 1.0;
     bool refused = false;
     while (true) {
         // The first position at or behind `a` that the binary32 sums do not
-        // accept for certain. A warp looks at one position; lanes 0-15 join
-        // the target row's parts, lanes 16-31 the draft row's.
+        // accept for certain. A half-warp joins the parts of its row.
         if (threadIdx.x == 0) sh.first = n;
         __syncthreads();
+        uint32_t at = 0;  // its warp
         for (uint32_t i0 = a; i0 < n; i0 += kDrawWarps) {
             const uint32_t i = i0 + warp;
             const bool mine = i < n;
-            const bool drafted = lane >= 16;
             float m = kNegInf;
             double s = 0.0;
             if (mine && (c.draft || !drafted) && (lane & 15u) < c.parts) {
@@ -425,103 +595,170 @@ verify_draw_kernel(const __grid_constant__ VerifyCall c, uint32_t ctas) {
                 s = part.sum;
             }
             sum_join_lanes(m, s, 16);
+            if (mine && i != warp) fetch(i, test_token, test_u, test_x);
+            const double e = fabsf(m) < kPosInf
+                                 ? exp64_or_zero(test_x, RowBase(c.scale, m), sh.tab)
+                                 : 0.0;
             const float mq = __shfl_sync(0xffffffffu, m, 16);
-            const double sq = __shfl_sync(0xffffffffu, s, 16);
+            const double sq = __shfl_sync(0xffffffffu, s, 16), eq = __shfl_sync(0xffffffffu, e, 16);
             if (mine && lane == 0) {
-                const uint32_t t = drafts[i];
                 bool certain = false;
                 const bool valid = fabsf(m) < kPosInf && (!c.draft || fabsf(mq) < kPosInf);
-                if (valid && t < c.vocab) {
-                    const double u = uniform_of(c, b, i, false);
-                    double left = u * s;
-                    double right = exp(static_cast<double>(masked_scaled(target_row(c, b, i)[t], c.scale)) - m);
-                    if (c.draft) {
-                        left *= exp(static_cast<double>(masked_scaled(draft_row(c, b, i)[t], c.scale)) - mq);
-                        right *= sq;
-                    }
-                    // Both sums are within 4e-6 of their values.
+                if (valid && test_token < c.vocab) {
+                    const double left = test_u * s * (c.draft ? eq : 1.0);
+                    const double right = e * (c.draft ? sq : 1.0);
+                    // Each sum is within 6e-6 of its value.
                     certain = left * (1.0 + 3e-5) < right;
                 }
                 if (!certain) atomicMin(&sh.first, i);
                 sh.max_p[warp] = m;
                 sh.max_q[warp] = mq;
+                sh.kappa[warp] = s / sq;
+                sh.test_u[warp] = test_u;
+                sh.test_p[warp] = test_x;
+                sh.test_token[warp] = test_token;
             }
+            if (mine && lane == 16) sh.test_q[warp] = test_x;
             __syncthreads();
             const uint32_t f = sh.first;
             if (f < n) {
-                if (threadIdx.x == 0) {
-                    sh.pos_max_p = sh.max_p[f - i0];
-                    sh.pos_max_q = sh.max_q[f - i0];
-                }
+                at = f - i0;
                 break;
             }
             __syncthreads();  // everyone has read sh.first
         }
-        __syncthreads();
         a = sh.first;
         refused = a < n;
         d.p = target_row(c, b, a);
-        float max_p = sh.pos_max_p, max_q = sh.pos_max_q;
         if (!refused) {
-            // The row behind the last test has no sums yet: its maximum first.
-            float m = kNegInf;
-            visit_segment<kDrawThreads, 4>(
-                d.p, lo, hi,
-                [&](uint32_t, uint32_t, const float4 *x) {
+            // The row behind the last test, of which nothing is known yet: each
+            // warp sums against the maximum of its first block; binary64 holds
+            // terms up to 600 above that, a run with larger ones is summed again.
+            float ref = kNegInf, top = kNegInf;
+            double s = 0.0;
+            while (true) {
+                visit_run<false, kRowLoads>(d.p, d.p, wlo, whi, [&](uint32_t, const float *x, const float *) {
+                    float m = x[0];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        m = fmaxf(fmaxf(m, fmaxf(x[k].x, x[k].y)), fmaxf(x[k].z, x[k].w));
-                },
-                [&](uint32_t, float x) { m = fmaxf(m, x); });
-            m = warp_max(masked_scaled(m, c.scale));
-            if (lane == 0) sh.warp_max[warp] = m;
-            __syncthreads();
-            if (threadIdx.x < ctas) {
-                for (int w = 0; w < kDrawWarps; ++w) m = fmaxf(m, sh.warp_max[w]);
-                cluster.map_shared_rank(&sh, threadIdx.x)->cta_max[rank] = m;
+                    for (int k = 1; k < kRowLoads; ++k) m = fmaxf(m, x[k]);
+                    m = masked_scaled(m, c.scale);
+                    top = fmaxf(top, m);
+                    if (ref == kNegInf) ref = warp_max(m);
+                    if (ref == kNegInf) return;  // nothing but -inf so far
+                    const RowBase base(c.scale, ref);
+#pragma unroll
+                    for (int k = 0; k < kRowLoads; ++k) s += exp64(x[k], base, sh.tab);
+                });
+                top = warp_max(top);
+                if (top == ref || !(top < kPosInf) || static_cast<double>(top) - ref <= 600.0) break;
+                ref = top;
+                s = 0.0;
             }
-            cluster.sync();
-            max_p = kNegInf;
-            for (uint32_t r = 0; r < ctas; ++r) max_p = fmaxf(max_p, sh.cta_max[r]);
+            s = warp_sum(s);
+            // On the CTA's largest reference.
+            if (lane == 0) {
+                sh.max_p[warp] = ref;
+                sh.max_q[warp] = top;
+            }
+            __syncthreads();
+            const float cta_ref = warp_max(lane < kDrawWarps ? sh.max_p[lane] : kNegInf);
+            const float cta_top = warp_max(lane < kDrawWarps ? sh.max_q[lane] : kNegInf);
+            s = ref == kNegInf ? 0.0 : s * exp(static_cast<double>(ref) - static_cast<double>(cta_ref));
+            share(s, warp == 0 ? static_cast<double>(cta_ref) : 0.0,
+                  warp == 0 ? static_cast<double>(cta_top) : 0.0, 0.0, 0u);
+            const double refs = lane < ctas ? sh.cta[set][lane].s[1] : -__longlong_as_double(0x7ff0000000000000ll);
+            const double row_ref = warp_max(refs);
+            const double row_top = warp_max(lane < ctas ? sh.cta[set][lane].s[2] : refs);
+            if (!(fabs(row_top) < __longlong_as_double(0x7ff0000000000000ll))) {
+                status = RSC_ROW_NO_VALID_TOKENS;
+                break;
+            }
+            d.weight = kWeightRow;
+            cta_weight = cta_sum(0) * (lane < ctas ? exp(refs - row_ref) : 0.0);
+            d.base_p = RowBase(c.scale, cta_ref);
+            own_scale = exp(row_ref - static_cast<double>(cta_ref));
+            if (threadIdx.x < kDrawWarps) sh.warp_weight[threadIdx.x] = sh.warp_sum[threadIdx.x][0];
+            total = warp_sum(cta_weight);
+            break;
         }
-        const bool paired = refused && c.draft;
+        const float max_p = sh.max_p[at], max_q = sh.max_q[at];
+        const double guess = sh.kappa[at];
+        const bool paired = c.draft != nullptr;
         if (!(fabsf(max_p) < kPosInf) || (paired && !(fabsf(max_q) < kPosInf))) {
             status = RSC_ROW_NO_VALID_TOKENS;
             break;
         }
-        d.max_p = max_p;
-        d.max_q = max_q;
-        d.without = refused ? drafts[a] : 0xffffffffu;
-        // Both rows' sums in binary64; without a draft row the second sum is
-        // that of the weights.
-        double s0 = 0.0, s1 = 0.0;
-        if (paired) d.q = draft_row(c, b, a);
-        for (uint32_t j = wlo + lane; j < whi; j += 32) {
-            const double e = exp64(static_cast<double>(masked_scaled(d.p[j], c.scale)) - d.max_p, sh.tab);
-            s0 += e;
-            if (paired)
-                s1 += exp64(static_cast<double>(masked_scaled(d.q[j], c.scale)) - d.max_q, sh.tab);
-            else
-                s1 += j == d.without ? 0.0 : e;
+        d.base_p = RowBase(c.scale, max_p);
+        d.base_q = RowBase(c.scale, max_q);
+        const uint32_t t = sh.test_token[at];
+        const float test_p = sh.test_p[at], test_q = sh.test_q[at];
+        const double u = sh.test_u[at];
+        d.without = t;
+        double s0 = 0.0, s1 = 0.0, s2 = 0.0, s3 = 0.0;
+        uint32_t n_near = 0;
+        if (paired) {
+            d.q = draft_row(c, b, a);
+            visit_run<true, kPairLoads>(d.p, d.q, wlo, whi, [&](uint32_t, const float *x, const float *y) {
+                double e[kPairLoads], f[kPairLoads];
+                bool any = false;
+#pragma unroll
+                for (int k = 0; k < kPairLoads; ++k) {
+                    e[k] = exp64(x[k], d.base_p, sh.tab);
+                    f[k] = exp64(y[k], d.base_q, sh.tab);
+                }
+#pragma unroll
+                for (int k = 0; k < kPairLoads; ++k) {
+                    s0 += e[k];
+                    s1 += f[k];
+                    const double g = guess * f[k], over = e[k] - g;
+                    // |over| <= 2^-16 g by the high words (up to their last bit).
+                    const int32_t high = __double2hiint(over);
+                    const bool near = (high & 0x7fffffff) + (16 << 20) <= __double2hiint(g) + 1;
+                    any |= near;
+                    if (high > 0 && !near) {
+                        s2 += over;
+                        s3 += f[k];
+                    }
+                }
+                if (__any_sync(0xffffffffu, any)) {
+#pragma unroll
+                    for (int k = 0; k < kPairLoads; ++k) {
+                        const double g = guess * f[k], over = e[k] - g;
+                        const bool near = e[k] > kNoWeight && (__double2hiint(over) & 0x7fffffff) + (16 << 20) <=
+                                                                  __double2hiint(g) + 1;
+                        const uint32_t who = __ballot_sync(0xffffffffu, near);
+                        const uint32_t slot = n_near + __popc(who & ((1u << lane) - 1u));
+                        if (near && slot < kNearWarp) {
+                            sh.warp_near[warp][slot][0] = e[k];
+                            sh.warp_near[warp][slot][1] = f[k];
+                        }
+                        n_near += __popc(who);
+                    }
+                }
+            });
+            s2 = warp_sum(s2);
+            s3 = warp_sum(s3);
+        } else {
+            visit_run<false, kRowLoads>(d.p, d.p, wlo, whi, [&](uint32_t j0, const float *x, const float *) {
+#pragma unroll
+                for (int k = 0; k < kRowLoads; ++k) {
+                    const double e = exp64(x[k], d.base_p, sh.tab);
+                    s0 += e;
+                    s1 += j0 + 32 * k + lane == t ? 0.0 : e;
+                }
+            });
         }
         s0 = warp_sum(s0);
         s1 = warp_sum(s1);
-        double sum_p, sum_1;
-        share_sums(s0, s1, sum_p, sum_1);
-        if (!refused) {
-            d.weight = kWeightRow;
-            total = sum_1;
-            break;
-        }
+        share(s0, s1, s2, s3, n_near);
+        const double sum_p = warp_sum(cta_sum(0)), sum_1 = warp_sum(cta_sum(1));
         // The exact decision.
-        const uint32_t t = drafts[a];
         bool accept = false;
         if (t < c.vocab) {
-            const double u = uniform_of(c, b, a, false);
             double left = u * sum_p;
-            double right = exp64(static_cast<double>(masked_scaled(d.p[t], c.scale)) - d.max_p, sh.tab);
+            double right = exp64_or_zero(test_p, d.base_p, sh.tab);
             if (paired) {
-                left *= exp64(static_cast<double>(masked_scaled(d.q[t], c.scale)) - d.max_q, sh.tab);
+                left *= exp64_or_zero(test_q, d.base_q, sh.tab);
                 right *= sum_1;
             }
             accept = left < right;
@@ -530,32 +767,45 @@ verify_draw_kernel(const __grid_constant__ VerifyCall c, uint32_t ctas) {
             ++a;
             continue;
         }
-        if (paired) {
-            d.weight = kWeightResidual;
-            d.inv_p = 1.0 / sum_p;
-            d.inv_q = 1.0 / sum_1;
-            double unused;
-            s1 = run_sum(d, wlo, whi, c.scale, sh.tab);
-            share_sums(0.0, s1, unused, total);
-        } else {
+        if (!paired) {
             d.weight = kWeightWithout;
-            total = sum_1;
+            cta_weight = cta_sum(1);
+            if (threadIdx.x < kDrawWarps) sh.warp_weight[threadIdx.x] = sh.warp_sum[threadIdx.x][1];
+            total = warp_sum(cta_weight);
+        } else {
+            d.weight = kWeightResidual;
+            d.kappa = sum_p / sum_1;
+            const bool many = lane < ctas && sh.cta[set][lane].n_near > kNearCta;
+            if (!__any_sync(0xffffffffu, many)) {
+                const double slip = guess - d.kappa;
+                cta_weight = lane < ctas ? residual_weight(cta_sum(2), cta_sum(3), slip, d.kappa,
+                                                           sh.cta[set][lane].near, sh.cta[set][lane].n_near)
+                                         : 0.0;
+                if (threadIdx.x < kDrawWarps)
+                    sh.warp_weight[threadIdx.x] = residual_weight(
+                        sh.warp_sum[threadIdx.x][2], sh.warp_sum[threadIdx.x][3], slip, d.kappa,
+                        sh.warp_near[threadIdx.x], sh.warp_n_near[threadIdx.x]);
+            } else {
+                share(run_sum(d, wlo, whi, sh.tab), 0.0, 0.0, 0.0, 0u);
+                cta_weight = cta_sum(0);
+                if (threadIdx.x < kDrawWarps) sh.warp_weight[threadIdx.x] = sh.warp_sum[threadIdx.x][0];
+            }
+            total = warp_sum(cta_weight);
         }
-        if (!(total > 0.0)) {
-            // p and q are equal and the token was outside both: p itself.
+        if (!(total > kNoWeight)) {
+            // Nothing is left (p and q are equal, the token was outside both): p itself.
             d.weight = kWeightRow;
-            double unused;
-            s1 = run_sum(d, wlo, whi, c.scale, sh.tab);
-            share_sums(0.0, s1, unused, total);
+            share(run_sum(d, wlo, whi, sh.tab), 0.0, 0.0, 0.0, 0u);
+            cta_weight = cta_sum(0);
+            if (threadIdx.x < kDrawWarps) sh.warp_weight[threadIdx.x] = sh.warp_sum[threadIdx.x][0];
+            total = warp_sum(cta_weight);
         }
         break;
     }
+    __syncthreads();  // warp_weight is complete
 
-    // The draw: the first index whose running weight exceeds u * total. The
-    // CTA whose share of the row holds it goes on alone: its warps' runs, then
-    // that run cut again, then one warp over what is left.
+    uint32_t *out = c.out_tokens + static_cast<size_t>(b) * (c.max_drafts + 1);
     if (rank == 0) {
-        uint32_t *out = c.out_tokens + static_cast<size_t>(b) * (c.max_drafts + 1);
         for (uint32_t i = threadIdx.x; i <= c.max_drafts; i += kDrawThreads)
             if (i != a) out[i] = i < a ? drafts[i] : 0xffffffffu;
         if (threadIdx.x == 0) {
@@ -564,88 +814,68 @@ verify_draw_kernel(const __grid_constant__ VerifyCall c, uint32_t ctas) {
             c.out_status[b] = status;
         }
     }
+    // The draw: the first index whose running weight exceeds u * total. The CTA
+    // whose share of the row holds it goes on alone: the run of one of its
+    // warps, cut again while it is longer than kTail elements a thread.
     const uint32_t tests = a + (refused ? 1u : 0u);
-    double want = 0.0;
     if (status == RSC_ROW_OK) {
-        want = static_cast<double>(uniform_of(c, b, tests, true)) * total;
-        double before = 0.0;
-        uint32_t owner = ctas, last = 0;
-        for (uint32_t r = 0; r < ctas; ++r) {
-            const double s = sh.cta_sum[set][r][1];
-            if (s > 0.0) last = r;
-            if (owner == ctas) {
-                if (before + s > want)
-                    owner = r;
-                else
-                    before += s;
-            }
-        }
-        // Rounding can leave u * total at the whole sum: then the last index
-        // of positive weight.
-        const bool past = owner == ctas;
-        if (past) owner = last;
-        if (owner == rank) {
-            double rest = past ? __longlong_as_double(0x7ff0000000000000ll) : want - before;
+        constexpr uint32_t kTail = 8;
+        double rest = static_cast<double>(c.uniforms ? last_u : uniform_of(c, b, tests, true)) * total;
+        if (locate(cta_weight, rest) == rank) {
+            rest *= own_scale;
             uint32_t flo = lo, fhi = hi;
             while (true) {
-                uint32_t w = kDrawWarps, end = 0;
-                double prior = 0.0;
-                for (int k = 0; k < kDrawWarps; ++k) {
-                    const double s = sh.warp_sum[k][1];
-                    if (s > 0.0) end = k;
-                    if (w == kDrawWarps) {
-                        if (prior + s > rest)
-                            w = k;
-                        else
-                            prior += s;
-                    }
-                }
-                if (w == kDrawWarps) {
-                    w = end;
-                    rest = __longlong_as_double(0x7ff0000000000000ll);
-                } else {
-                    rest -= prior;
-                }
+                const uint32_t w = locate(lane < kDrawWarps ? sh.warp_weight[lane] : 0.0, rest);
                 uint32_t nlo, nhi;
                 warp_run(flo, fhi, w, nlo, nhi);
                 flo = nlo;
                 fhi = nhi;
-                if (fhi - flo <= 256) break;
+                if (fhi - flo <= kTail * kDrawThreads) break;
                 warp_run(flo, fhi, warp, nlo, nhi);
-                const double s = run_sum(d, nlo, nhi, c.scale, sh.tab);
+                const double s = run_sum(d, nlo, nhi, sh.tab);
                 __syncthreads();
-                if (lane == 0) sh.warp_sum[warp][1] = s;
+                if (lane == 0) sh.warp_weight[warp] = s;
                 __syncthreads();
             }
-            if (warp == 0) {
-                uint32_t token = 0xffffffffu, positive = 0xffffffffu;
-                double run = 0.0;
-                for (uint32_t j0 = flo; j0 < fhi && token == 0xffffffffu; j0 += 32) {
-                    const uint32_t j = j0 + lane;
-                    const double w = j < fhi ? weight_at(d, j, c.scale, sh.tab) : 0.0;
-                    double cum = w;
+            const uint32_t each = (fhi - flo + kDrawThreads - 1) / kDrawThreads;
+            const uint32_t j0 = flo + threadIdx.x * each;
+            double w[kTail], sum = 0.0;
 #pragma unroll
-                    for (int o = 1; o < 32; o *= 2) {
-                        const double up = __shfl_up_sync(0xffffffffu, cum, o);
-                        if (lane >= static_cast<uint32_t>(o)) cum += up;
-                    }
-                    cum += run;
-                    const uint32_t pos = __ballot_sync(0xffffffffu, w > 0.0);
-                    const uint32_t hit = __ballot_sync(0xffffffffu, w > 0.0 && cum > rest);
-                    if (pos) positive = j0 + 31u - __clz(pos);
-                    if (hit) token = j0 + __ffs(hit) - 1u;
-                    run = __shfl_sync(0xffffffffu, cum, 31);
+            for (uint32_t k = 0; k < kTail; ++k) {
+                const uint32_t j = j0 + k;
+                w[k] = 0.0;
+                if (k < each && j < fhi) {
+                    w[k] = weight_of(d, j, d.p[j], d.weight == kWeightResidual ? d.q[j] : 0.0f, sh.tab);
+                    if (!(w[k] > kNoWeight)) w[k] = 0.0;
                 }
-                if (lane == 0)
-                    c.out_tokens[static_cast<size_t>(b) * (c.max_drafts + 1) + a] =
-                        token != 0xffffffffu ? token : positive;
+                sum += w[k];
+            }
+            const double upto = warp_scan(sum);
+            __syncthreads();
+            if (lane == 31) sh.warp_weight[warp] = upto;
+            __syncthreads();
+            if (locate(lane < kDrawWarps ? sh.warp_weight[lane] : 0.0, rest) == warp &&
+                locate(sum, rest) == lane) {
+                double run = 0.0;
+                uint32_t token = j0;
+                bool found = false;
+#pragma unroll
+                for (uint32_t k = 0; k < kTail; ++k) {
+                    if (found || w[k] == 0.0) continue;
+                    run += w[k];
+                    token = j0 + k;
+                    found = run > rest;
+                }
+                out[a] = token;
             }
         }
     }
-    // Every CTA has taken its uniforms and its peers' sums.
-    cluster.sync();
-    if (c.rng_states && !c.uniforms && rank == 0 && threadIdx.x == 0)
-        c.rng_states[b] += kWyInc * static_cast<uint64_t>(status == RSC_ROW_OK ? tests + 1u : a);
+    if (c.rng_states) {
+        // Every CTA has taken its draws from the state.
+        cluster.sync();
+        if (rank == 0 && threadIdx.x == 0)
+            c.rng_states[b] += kWyInc * static_cast<uint64_t>(status == RSC_ROW_OK ? tests + 1u : a);
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -796,18 +1026,33 @@ verify_records_kernel(const __grid_constant__ VerifyCall c) {
 
 }  // namespace
 
+// Parts of a row. A batch whose rows are fewer than the CTAs that fit the GPU
+// at once (six per SM) is spread over one wave of them, in parts of at least
+// 2048 logits; a larger one is cut into parts of about 32768.
 uint32_t verify_parts(size_t rows, uint32_t vocab, int num_sms) {
-    // Enough CTAs for six per SM, in parts of at least 2048 logits.
-    const size_t want = static_cast<size_t>(num_sms) * 6;
-    uint32_t parts = 1;
-    while (parts < kVerifyMaxParts && rows * parts < want && vocab / (parts * 2) >= 2048) parts *= 2;
-    return parts;
+    const size_t wave = static_cast<size_t>(num_sms) * 6;
+    size_t parts = rows < wave ? wave / (rows ? rows : 1) : 1;
+    parts = std::max<size_t>(parts, (static_cast<size_t>(vocab) + 32767) / 32768);
+    parts = std::min<size_t>(parts, std::max<uint32_t>(1u, vocab / 2048));
+    return static_cast<uint32_t>(std::min<size_t>(parts, kVerifyMaxParts));
 }
 
 size_t verify_workspace_bytes(size_t n_seqs, size_t max_drafts, size_t vocab) {
-    size_t parts = 1;
-    while (parts < kVerifyMaxParts && vocab / (parts * 2) >= 2048) parts *= 2;
+    const size_t parts = std::min<size_t>(kVerifyMaxParts, std::max<size_t>(1, vocab / 2048));
     return n_seqs * (2 * max_drafts + 1) * parts * sizeof(RowPart);
+}
+
+// CTAs a sequence is drawn by. Few sequences take as many as leave the GPU's
+// SMs one or two each (16 is the largest cluster, above 8 only where the whole
+// of it finds room); more take slices of about 24576 tokens, whose uneven
+// lengths (a refused token reads two rows, an accepted draft one) even out.
+// Measured, us a call: 8 x 5 x 151936 27.5 with 16 CTAs, 35.7 with 8; 32 x 8 x
+// 50001 20.5 with 6, 25.8 with 8; 96 x 7 x 128256 123 with 6, 138 with 2.
+uint32_t draw_ctas(uint32_t n_seqs, uint32_t vocab, int num_sms) {
+    const uint32_t room = static_cast<uint32_t>(num_sms) * 4u / 3u / n_seqs;
+    uint32_t ctas = room >= 16 ? 16u : std::min(room, 8u);
+    ctas = std::max(ctas, std::min(8u, (vocab + 24575u) / 24576u));
+    return std::max(1u, std::min(ctas, vocab / 1024u));
 }
 
 cudaError_t launch_verify(const VerifyCall &call, bool greedy, int num_sms, uint64_t *launches,
@@ -842,12 +1087,14 @@ cudaError_t launch_verify(const VerifyCall &call, bool greedy, int num_sms, uint
         cfg.numAttrs = row_count > 0 ? 1 : 0;
         return cudaLaunchKernelEx(&cfg, verify_greedy_kernel, c);
     }
-    uint32_t ctas = 1;
-    while (ctas < kDrawMaxCtas && static_cast<size_t>(c.n_seqs) * ctas < 2u * num_sms &&
-           c.vocab / (ctas * 2) >= 2048)
-        ctas *= 2;
+    const uint32_t ctas = draw_ctas(c.n_seqs, c.vocab, num_sms);
+    if (ctas > 8) {
+        e = cudaFuncSetAttribute(verify_draw_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return e;
+    }
     cfg.gridDim = dim3(c.n_seqs * ctas, 1, 1);
     cfg.blockDim = dim3(kDrawThreads, 1, 1);
+    cfg.dynamicSmemBytes = sizeof(DrawShared);
     attr[1].id = cudaLaunchAttributeClusterDimension;
     attr[1].val.clusterDim.x = ctas;
     attr[1].val.clusterDim.y = 1;
