@@ -254,6 +254,8 @@ rsc_status rsc_sampler_create(int device, size_t max_rows, size_t max_vocab, rsc
     if (e == cudaSuccess) e = cudaMalloc(&s->stage_status, s->max_rows * sizeof(int32_t));
     if (e == cudaSuccess) e = cudaMalloc(&s->stage_probs, s->max_rows * sizeof(float));
     if (e == cudaSuccess) e = cudaStreamCreateWithFlags(&s->host_stream, cudaStreamNonBlocking);
+    if (e == cudaSuccess) e = rsc::verify_setup();
+    if (e == cudaSuccess) e = rsc::distill_setup();
     if (e != cudaSuccess) {
         s->alive = true;
         rsc_sampler_destroy(s);
@@ -867,7 +869,8 @@ rsc_status check_distill(const rsc_sampler *s, const rsc_distill_batch *x, const
     if (x->dtype != RSC_F32 && x->dtype != RSC_BF16 && x->dtype != RSC_F16)
         return RSC_ERR_INVALID_ARGUMENT;
     const float scale = 1.0f / x->temperature;
-    if (!(x->temperature > 0.0f) || !std::isfinite(scale) || !(scale > 0.0f))
+    // (The exponents are taken with 1/T log2(e).)
+    if (!(x->temperature > 0.0f) || !std::isfinite(scale * 1.44269504f) || !(scale > 0.0f))
         return RSC_ERR_INVALID_ARGUMENT;
     if (x->rows == 0) return RSC_OK;
     if (x->vocab == 0) return RSC_ERR_INVALID_SHAPE;

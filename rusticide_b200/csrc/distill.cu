@@ -19,6 +19,9 @@
 // lose it where the listed tokens hold nearly all of the mass. Sums leave a
 // thread's batch of 16 in binary64 (rsc_rowsum.cuh), what is computed per row
 // or per entry is binary64 throughout.
+#include <algorithm>
+#include <type_traits>
+
 #include <cooperative_groups.h>
 
 #include "rsc_common.cuh"
@@ -37,26 +40,39 @@ constexpr uint32_t kMaxCtas = 8;  // the largest portable cluster
 constexpr uint32_t kLoads = 4;    // 16-byte loads in flight per thread
 
 // One CTA's contribution to its row, shared with the whole cluster.
-struct RowShare {
-    float max_rest, max_listed;  // over the tokens summed in the pass; over the listed ones
-    double sum_rest, sum_listed;
-    double cross, held;  // sums of t (log t - v) and of t over the CTA's entries
+struct __align__(16) RowShare {
+    float max_rest, sum_rest;      // over the tokens of the pass
+    float max_listed, sum_listed;  // over the listed ones, with the tail
+    double cross, held;            // sums of t (y - y_ref - v) and of t over the CTA's entries
 };
 
 struct DistillShared {
-    uint32_t id[kDistillMaxTop];
-    float t[kDistillMaxTop];  // teacher probability
-    float v[kDistillMaxTop];  // scaled student logit (entries of this CTA's segment)
-    float y[kDistillMaxTop];  // teacher log-probability as given
-    float red_m[kWarps];
-    double red_s[kWarps];
+    float red_m[kWarps], red_s[kWarps];
+    float list_m[kWarps], list_s[kWarps];
+    float red_y[kWarps];
+    double red_t[kWarps];
     RowShare share[kMaxCtas];
-    double log_norm;  // log t = y - log_norm
+    uint32_t unordered;
+    float4 row;  // maximum, 1 / sum, unlisted maximum, unlisted factor
+};
+
+// A row's teacher entries in shared memory (cap of each).
+struct Entries {
+    uint32_t *id;
+    float *y;  // log-probability as given
+    float *t;  // probability
+    float *v;  // scaled student logit (entries of this CTA's segment)
+};
+__device__ __forceinline__ uint32_t list_warps(uint32_t n) { return min(static_cast<uint32_t>(kWarps), (n + 31u) / 32u); }
+constexpr size_t kEntryBytes = 16;
+
+// What is known of a row's list as a whole, in every thread.
+struct Teacher {
+    uint32_t n;
+    bool some;         // it has an entry
+    float y_ref;       // what exponents were taken against
+    double sum;        // of exp(y - y_ref)
     double r, mass;
-    uint32_t some, unordered;
-    // The row as the gradient needs it: p = exp(v - max) * inv on the listed
-    // tokens, exp(v - rest_max) * rest_factor the whole term on the others.
-    float max, inv, rest_max, rest_factor;
 };
 
 template <typename T>
@@ -70,77 +86,222 @@ __device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) {
 template <>
 __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 
+// Exponentials of a row against a reference value `ref` (any number near its
+// largest v): exp(v - ref) = 2^(x c - mc) * 2^-slip with c = fl(s log2 e) and mc =
+// fl(ref log2 e), one packed multiply-add for two of them. The exponent is
+// rounded once and c carries 2^-24 of it, |v - ref| 2^-22 in all; what mc and c
+// make the reference off by is the same factor for the whole row, slip (log2,
+// binary64), and is taken out of sums and factors. Where ref log2 e leaves
+// binary32 (`wide`) the exponent is (v - ref) log2 e instead.
+struct ExpRef {
+    float ref, c, mc;
+    bool wide;
+    __device__ __forceinline__ ExpRef(const DistillCall &call, float ref_)
+        : ref(ref_), c(call.exp2_scale), mc(ref_ * 1.44269504f) {
+        wide = !(fabsf(mc) < kPosInf) && fabsf(ref) < kPosInf;
+    }
+    // 2^-slip, which a sum or factor of these exponentials is to be multiplied by.
+    __device__ __forceinline__ double correction(const DistillCall &call) const {
+        if (wide) return 1.0;
+        const double z = -0.6931471805599453 *
+                         __fma_rn(static_cast<double>(ref), call.exp2_ratio, -static_cast<double>(mc));
+        // |z| is 1e-7 of |ref|; its cube / 6 is below 2e-13 in the short form.
+        return fabs(z) < 1e-4 ? __fma_rn(z, __fma_rn(z, 0.5, 1.0), 1.0) : exp(z);
+    }
+};
+
+__device__ __forceinline__ float ex2_fast(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// Two binary32 values in one 64-bit register pair, as the packed operations
+// take them.
+__device__ __forceinline__ uint64_t pair_of(float a, float b) {
+    uint64_t p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+    return p;
+}
+__device__ __forceinline__ float low_of(uint64_t p) {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+    return a;
+}
+__device__ __forceinline__ float high_of(uint64_t p) {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+    return b;
+}
+// The largest of a warp's values (NaN passed over), in every lane.
+__device__ __forceinline__ float warp_top(float v) {
+    float r;
+    asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma_pair(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add_pair(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// Two neighbouring exponentials.
+__device__ __forceinline__ uint64_t exp_pair(uint64_t x, uint64_t c, uint64_t minus_mc) {
+    const uint64_t t = fma_pair(x, c, minus_mc);
+    return pair_of(ex2_fast(low_of(t)), ex2_fast(high_of(t)));
+}
+__device__ __forceinline__ float exp_one(float x, float scale, const ExpRef &r) {
+    return r.wide ? exp_fast(__fsub_rn(__fmul_rn(x, scale), r.ref))
+                  : ex2_fast(__fmaf_rn(x, r.c, -r.mc));
+}
+
+// The largest element of a 16-byte word (NaN passed over).
+template <typename T>
+__device__ __forceinline__ float word_max(const uint4 &w);
+template <>
+__device__ __forceinline__ float word_max<float>(const uint4 &w) {
+    return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)),
+                 fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+}
+template <>
+__device__ __forceinline__ float word_max<__nv_bfloat16>(const uint4 &w) {
+    const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&w);
+    const __nv_bfloat162 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+template <>
+__device__ __forceinline__ float word_max<__half>(const uint4 &w) {
+    const __half2 *h = reinterpret_cast<const __half2 *>(&w);
+    const __half2 m = __hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3]));
+    return fmaxf(__low2float(m), __high2float(m));
+}
+
+// A 16-byte word of the gradient from one of the logits: exp(v - ref) * factor.
+template <typename T, bool kWide>
+__device__ __forceinline__ uint4 grad_word(const uint4 &w, float scale, const ExpRef &r, float factor) {
+    constexpr int kE = kVecElems<T>;
+    float v[kE];
+    unpack<T>(w, v);
+    union {
+        uint4 word;
+        T elem[kE];
+    } o;
+#pragma unroll
+    for (int i = 0; i < kE; i += 2) {
+        if (kWide) {
+            o.elem[i] = from_float<T>(__fmul_rn(exp_one(v[i], scale, r), factor));
+            o.elem[i + 1] = from_float<T>(__fmul_rn(exp_one(v[i + 1], scale, r), factor));
+        } else {
+            const uint64_t g = mul_pair(exp_pair(pair_of(v[i], v[i + 1]), pair_of(r.c, r.c), pair_of(-r.mc, -r.mc)),
+                                        pair_of(factor, factor));
+            o.elem[i] = from_float<T>(low_of(g));
+            o.elem[i + 1] = from_float<T>(high_of(g));
+        }
+    }
+    return o.word;
+}
+
 // The id of an absent entry: one outside the vocabulary, or of no probability.
 constexpr uint32_t kAbsent = 0xffffffffu;
 
-// The teacher's list of a row: ids, t and the sums over them.
-__device__ __forceinline__ uint32_t load_teacher(const DistillCall &c, size_t row, DistillShared &sh) {
-    uint32_t n = static_cast<uint32_t>(c.cap);
-    if (c.n) n = min(n, c.n[row]);
-    for (uint32_t k = threadIdx.x; k < n; k += kThreads) {
-        const uint32_t id = c.ids[row * c.cap + k];
-        const float y = c.logprobs[row * c.cap + k];
-        sh.id[k] = id < c.vocab && y != kNegInf ? id : kAbsent;
-        sh.y[k] = y;
-    }
+// The teacher's list of a row, one entry a thread for lists of up to a block.
+// The exponentials are binary64: with the tail, r is what they leave of 1.
+__device__ __forceinline__ Teacher load_teacher(const DistillCall &c, size_t row, const Entries &e,
+                                                DistillShared &sh) {
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    Teacher te;
+    te.n = static_cast<uint32_t>(c.cap);
+    if (c.n) te.n = min(te.n, c.n[row]);
+    const uint32_t n = te.n, warps = list_warps(n);
     if (threadIdx.x == 0) sh.unordered = 0;
-    __syncthreads();
-    // Lists in ascending order hold no id twice.
-    for (uint32_t k = threadIdx.x; k + 1 < n; k += kThreads)
-        if (!(sh.id[k] < sh.id[k + 1]) && sh.id[k + 1] != kAbsent) sh.unordered = 1;
-    if (threadIdx.x < 32) {
-        float top = kNegInf;
-        bool some = false;
-        for (uint32_t k = threadIdx.x; k < n; k += 32)
-            if (sh.id[k] != kAbsent) {
-                top = fmaxf(top, sh.y[k]);
-                some = true;
-            }
-        top = warp_max(top);
-        some = __any_sync(0xffffffffu, some);
-        // With the tail the values are log-probabilities as such.
-        const double ref = c.tail || !(fabsf(top) < kPosInf) ? 0.0 : static_cast<double>(top);
-        double sum = 0.0;
-        for (uint32_t k = threadIdx.x; k < n; k += 32)
-            if (sh.id[k] != kAbsent) sum += exp(static_cast<double>(sh.y[k]) - ref);
-        sum = warp_sum(sum);
-        if (threadIdx.x == 0) {
-            sh.some = some ? 1u : 0u;
-            if (c.tail) {
-                sh.log_norm = 0.0;
-                sh.r = sum < 1.0 ? 1.0 - sum : 0.0;
-                sh.mass = sum > 1.0 ? sum : 1.0;
-            } else {
-                sh.log_norm = ref + log(sum);
-                sh.r = 0.0;
-                sh.mass = 1.0;
-            }
+    float top = kNegInf;
+    bool some = false, unordered = false;
+    for (uint32_t k = threadIdx.x; k < n; k += kThreads) {
+        const uint32_t *ids = c.ids + row * c.cap;
+        const uint32_t id = ids[k], next = k + 1 < n ? ids[k + 1] : kAbsent;
+        const float y = c.logprobs[row * c.cap + k];
+        const bool there = id < c.vocab && y != kNegInf;
+        e.id[k] = there ? id : kAbsent;
+        e.y[k] = y;
+        // Lists in ascending order (padding aside) hold no id twice.
+        unordered |= !(id < next) && next < c.vocab;
+        some |= there;
+        if (there) top = fmaxf(top, y);
+    }
+    te.some = __syncthreads_or(some);
+    if (unordered) sh.unordered = 1;
+    // With the tail the values are log-probabilities as such.
+    te.y_ref = 0.0f;
+    if (!c.tail) {
+        if (warp < warps) {
+            top = warp_top(top);
+            if (lane == 0) sh.red_y[warp] = top;
         }
+        __syncthreads();
+        top = sh.red_y[0];
+        for (uint32_t w = 1; w < warps; ++w) top = fmaxf(top, sh.red_y[w]);
+        if (fabsf(top) < kPosInf) te.y_ref = top;
+    }
+    if (warp < warps) {
+        double part = 0.0;
+        for (uint32_t k = threadIdx.x; k < n; k += kThreads) {
+            const double p = e.id[k] != kAbsent
+                                 ? exp(static_cast<double>(e.y[k]) - static_cast<double>(te.y_ref)) : 0.0;
+            e.t[k] = static_cast<float>(p);
+            part += p;
+        }
+        part = warp_sum(part);
+        if (lane == 0) sh.red_t[warp] = part;
     }
     __syncthreads();
-    for (uint32_t k = threadIdx.x; k < n; k += kThreads)
-        sh.t[k] = sh.id[k] != kAbsent
-                      ? static_cast<float>(exp(static_cast<double>(sh.y[k]) - sh.log_norm))
-                      : 0.0f;
-    return n;
+    te.sum = 0.0;
+    for (uint32_t w = 0; w < warps; ++w) te.sum += sh.red_t[w];
+    te.r = 0.0;
+    te.mass = 1.0;
+    if (c.tail) {
+        if (te.sum < 1.0) te.r = 1.0 - te.sum;
+        if (te.sum > 1.0) te.mass = te.sum;
+    } else if (warp < warps) {
+        const float inv = __fdiv_rn(1.0f, static_cast<float>(te.sum));
+        for (uint32_t k = threadIdx.x; k < n; k += kThreads) e.t[k] = __fmul_rn(e.t[k], inv);
+    }
+    return te;
 }
 
 // Entry k is the first of its id, and the sum of t over the entries of that
 // id in list order (ids may repeat: each entry counts).
-__device__ __forceinline__ bool first_of_id(const DistillShared &sh, uint32_t n, uint32_t k,
+__device__ __forceinline__ bool first_of_id(const Entries &e, bool unordered, uint32_t n, uint32_t k,
                                             float &t_sum) {
-    t_sum = sh.t[k];
-    if (!sh.unordered) return true;
-    const uint32_t id = sh.id[k];
+    t_sum = e.t[k];
+    if (!unordered) return true;
+    const uint32_t id = e.id[k];
     double sum = 0.0;
     bool first = true;
     for (uint32_t q = 0; q < n; ++q) {
-        if (sh.id[q] != id) continue;
+        if (e.id[q] != id) continue;
         first &= q >= k;
-        sum += static_cast<double>(sh.t[q]);
+        sum += static_cast<double>(e.t[q]);
     }
     t_sum = static_cast<float>(sum);
     return first;
+}
+
+// The (m, s) pairs of a warp's lanes joined in binary32, in all of them. A sum
+// against -inf is 0 or NaN and stays.
+__device__ __forceinline__ void join_lanes(float &m, float &s) {
+    const float top = warp_top(m);
+    if (m != kNegInf) s = __fmul_rn(s, exp_fast(__fsub_rn(m, top)));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, o));
+    m = top;
 }
 
 // A row segment of T cut at 16-byte boundaries: [lo, body) and [tail, hi)
@@ -158,12 +319,175 @@ struct Segment {
     }
 };
 
-template <typename T, bool kForward, bool kGrad>
-__global__ void __launch_bounds__(kThreads)
-distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas) {
-    extern __shared__ uint32_t bits[];  // one per element of the segment, set where it is listed
-    __shared__ DistillShared sh;
+// The exponentials of kN 16-byte words added up as a tree.
+template <typename T, int kN>
+__device__ __forceinline__ float batch_sum(const uint4 *w, uint64_t c, uint64_t minus_mc) {
+    constexpr int kE = kVecElems<T>, kPairs = kN * kE / 2;
+    uint64_t e[kPairs];
+#pragma unroll
+    for (int k = 0; k < kN; ++k) {
+        float v[kE];
+        unpack<T>(w[k], v);
+#pragma unroll
+        for (int i = 0; i < kE; i += 2) e[(k * kE + i) / 2] = exp_pair(pair_of(v[i], v[i + 1]), c, minus_mc);
+    }
+#pragma unroll
+    for (int d = 1; d < kPairs; d *= 2) {
+#pragma unroll
+        for (int i = 0; i + d < kPairs; i += 2 * d) e[i] = add_pair(e[i], e[i + d]);
+    }
+    return __fadd_rn(low_of(e[0]), high_of(e[0]));
+}
+
+// (m, s) of this thread's share of a segment in shared memory, src[j] the
+// element j: the maximum first, then the exponentials against it.
+template <typename T>
+__device__ __forceinline__ void sum_resident(const DistillCall &c, const T *src, const Segment<T> &seg,
+                                             float &m, double &s) {
+    constexpr int kE = kVecElems<T>;
+    const uint4 *words = reinterpret_cast<const uint4 *>(src + seg.body);
+    const bool head = threadIdx.x < seg.body - seg.lo;
+    const bool tail = threadIdx.x >= 32 && threadIdx.x - 32 < seg.hi - seg.tail;
+    float top = kNegInf;
+    for (uint32_t q = threadIdx.x; q < seg.n_vec; q += kThreads) top = fmaxf(top, word_max<T>(words[q]));
+    const float one = head ? elem_to_float<T>(src[seg.lo + threadIdx.x])
+                           : tail ? elem_to_float<T>(src[seg.tail + threadIdx.x - 32]) : kNegInf;
+    top = fmaxf(top, one);
+    m = __fmul_rn(top, c.scale);
+    const ExpRef r(c, top == kNegInf ? 0.0f : m);
+    s = static_cast<double>(exp_one(one, c.scale, r));
+    if (r.wide) {
+        for (uint32_t q = threadIdx.x; q < seg.n_vec; q += kThreads) {
+            float v[kE];
+            unpack<T>(words[q], v);
+            for (int i = 0; i < kE; ++i) s += static_cast<double>(exp_one(v[i], c.scale, r));
+        }
+        return;
+    }
+    const uint64_t cc = pair_of(r.c, r.c), mc = pair_of(-r.mc, -r.mc);
+    uint32_t q0 = threadIdx.x;
+    for (; q0 + kThreads * (kLoads - 1) < seg.n_vec; q0 += kThreads * kLoads) {
+        uint4 w[kLoads];
+#pragma unroll
+        for (uint32_t k = 0; k < kLoads; ++k) w[k] = words[q0 + k * kThreads];
+        s += static_cast<double>(batch_sum<T, kLoads>(w, cc, mc));
+    }
+    for (; q0 < seg.n_vec; q0 += kThreads) s += static_cast<double>(batch_sum<T, 1>(words + q0, cc, mc));
+    s *= r.correction(c);
+}
+
+// (m, s) of this thread's share of a segment in global memory: a batch of
+// 16-byte words at a time against one running maximum. Where the tail is wanted
+// by itself the listed elements are left out by their bit.
+template <typename T>
+__device__ __forceinline__ void sum_streamed(const DistillCall &c, const T *x, const Segment<T> &seg,
+                                             uint32_t *bits, const Entries &en, uint32_t n, float &m,
+                                             double &s) {
     constexpr uint32_t kE = kVecElems<T>;
+    const uint32_t lo = seg.lo, hi = seg.hi;
+    const bool masked = c.tail;
+    // Bit b stands for element lo - pad + b, so that the words' elements start at
+    // bit 32 * first.
+    const uint32_t first = (seg.body - lo + 31u) / 32u;
+    const uint32_t pad = first * 32u - (seg.body - lo);
+    if (masked) {
+        for (uint32_t w = threadIdx.x; w < (hi - lo + pad + 31u) / 32u; w += kThreads) bits[w] = 0;
+        __syncthreads();
+        for (uint32_t k = threadIdx.x; k < n; k += kThreads)
+            if (en.id[k] >= lo && en.id[k] < hi) {
+                const uint32_t b = en.id[k] - lo + pad;
+                atomicOr(&bits[b / 32u], 1u << (b % 32u));
+            }
+        __syncthreads();
+    }
+    const unsigned char *bytes = reinterpret_cast<const unsigned char *>(bits + first);
+    // This thread's element of the head or tail, if it has one.
+    float one = kNegInf;
+    uint32_t j = hi;
+    if (threadIdx.x < seg.body - lo) j = lo + threadIdx.x;
+    if (threadIdx.x >= 32 && threadIdx.x - 32 < hi - seg.tail) j = seg.tail + threadIdx.x - 32;
+    if (j < hi && !(masked && (bits[(j - lo + pad) / 32u] >> ((j - lo + pad) % 32u) & 1u)))
+        one = elem_to_float<T>(x[j]);
+    float top = one;
+    ExpRef r(c, top > kNegInf ? __fmul_rn(top, c.scale) : 0.0f);
+    double correction = r.correction(c);
+    s = static_cast<double>(exp_one(one, c.scale, r)) * correction;
+    const uint4 *words = reinterpret_cast<const uint4 *>(x + seg.body);
+    // A batch of words, the listed elements among them taken out.
+    auto add = [&](uint4 *w, const uint32_t *set, auto count) {
+        constexpr int kN = decltype(count)::value;
+        uint32_t any = 0;
+#pragma unroll
+        for (int k = 0; k < kN; ++k) any |= set[k];
+        if (any) {
+#pragma unroll
+            for (int k = 0; k < kN; ++k) {
+                union {
+                    uint4 word;
+                    T elem[kE];
+                } u;
+                u.word = w[k];
+#pragma unroll
+                for (uint32_t i = 0; i < kE; ++i)
+                    if (set[k] >> i & 1u) u.elem[i] = from_float<T>(kNegInf);
+                w[k] = u.word;
+            }
+        }
+        float b = word_max<T>(w[0]);
+#pragma unroll
+        for (int k = 1; k < kN; ++k) b = fmaxf(b, word_max<T>(w[k]));
+        if (b > top) {
+            const float next = __fmul_rn(b, c.scale);
+            // Before the first logit above -inf the sum is 0 or NaN.
+            if (top > kNegInf) s *= static_cast<double>(exp_fast(__fsub_rn(r.ref, next)));
+            top = b;
+            r = ExpRef(c, next);
+            correction = r.correction(c);
+        }
+        if (r.wide) {
+            for (int k = 0; k < kN; ++k) {
+                float v[kE];
+                unpack<T>(w[k], v);
+                for (uint32_t i = 0; i < kE; ++i) s += static_cast<double>(exp_one(v[i], c.scale, r));
+            }
+        } else {
+            s += static_cast<double>(batch_sum<T, kN>(w, pair_of(r.c, r.c), pair_of(-r.mc, -r.mc))) * correction;
+        }
+    };
+    auto listed = [&](uint32_t q) -> uint32_t {
+        if (!masked) return 0u;
+        return kE == 8 ? bytes[q] : bytes[q / 2u] >> (4u * (q & 1u)) & 15u;
+    };
+    uint32_t q0 = threadIdx.x;
+    for (; q0 + kThreads * (kLoads - 1) < seg.n_vec; q0 += kThreads * kLoads) {
+        uint4 w[kLoads];
+        uint32_t set[kLoads];
+#pragma unroll
+        for (uint32_t k = 0; k < kLoads; ++k) w[k] = __ldg(words + q0 + k * kThreads);
+#pragma unroll
+        for (uint32_t k = 0; k < kLoads; ++k) set[k] = listed(q0 + k * kThreads);
+        add(w, set, std::integral_constant<int, kLoads>());
+    }
+    for (; q0 < seg.n_vec; q0 += kThreads) {
+        uint4 w = __ldg(words + q0);
+        const uint32_t set = listed(q0);
+        add(&w, &set, std::integral_constant<int, 1>());
+    }
+    m = top > kNegInf ? r.ref : kNegInf;
+}
+
+// kResident: the CTA's segment is copied to shared memory once (1-D TMA bulk
+// copies) and read there by both passes, so a row crosses HBM once for the loss
+// and once more for the gradient's write; listed elements are overwritten with
+// -inf there instead of being looked up in a bitmap.
+template <typename T, bool kForward, bool kGrad, bool kResident>
+__global__ void __launch_bounds__(kThreads)
+distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t buffer_bytes) {
+    // The first buffer_bytes: the segment, in the 16-byte phase of its global
+    // address (resident), or one bit per element of it. Then the entries.
+    extern __shared__ __align__(16) unsigned char dynamic[];
+    __shared__ DistillShared sh;
+    __shared__ uint64_t bar;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t rank = cluster.block_rank();
     const size_t row = blockIdx.x / ctas;
@@ -172,238 +496,265 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas) {
     const uint32_t seg_len = ((c.vocab + ctas - 1) / ctas + 31u) & ~31u;
     const uint32_t lo = min(c.vocab, rank * seg_len), hi = min(c.vocab, lo + seg_len);
     const Segment<T> seg(x, lo, hi);
-    const uint32_t n = load_teacher(c, row, sh);
+    Entries e;
+    e.id = reinterpret_cast<uint32_t *>(dynamic + buffer_bytes);
+    e.y = reinterpret_cast<float *>(e.id + c.cap);
+    e.t = e.y + c.cap;
+    e.v = e.t + c.cap;
+    // src[j]: element j, from where both passes read it.
+    const T *src = x;
+    T *held = nullptr;
+    bool copied = false;
+    if (kResident) {
+        held = reinterpret_cast<T *>(dynamic + (reinterpret_cast<uintptr_t>(x + lo) & 15u)) - lo;
+        src = held;
+        // An empty list needs no logits.
+        copied = c.cap > 0 && !(c.n && c.n[row] == 0);
+        if (threadIdx.x == 0) {
+            mbar_init(&bar, 1);
+            fence_barrier_init();
+            if (copied) {
+                mbar_arrive_expect_tx(&bar, seg.n_vec * 16u);
+                constexpr uint32_t kCopy = 1024;  // 16 KiB each
+                for (uint32_t q = 0; q < seg.n_vec; q += kCopy)
+                    tma_load_1d(held + seg.body + q * kVecElems<T>, x + seg.body + q * kVecElems<T>,
+                                min(kCopy, seg.n_vec - q) * 16u, &bar);
+            }
+        }
+        if (copied) {
+            if (threadIdx.x < seg.body - lo) held[lo + threadIdx.x] = x[lo + threadIdx.x];
+            if (threadIdx.x >= 32 && threadIdx.x - 32 < hi - seg.tail)
+                held[seg.tail + threadIdx.x - 32] = x[seg.tail + threadIdx.x - 32];
+        }
+    }
+    const Teacher te = load_teacher(c, row, e, sh);
+    const uint32_t n = te.n;
+    const bool empty = !te.some;
     // Every CTA of the cluster runs before its memory is written (the row is
     // empty for all of them or for none).
-    if (kForward && sh.some) cluster.barrier_arrive();
+    if (kForward && !empty) cluster.barrier_arrive();
     auto here = [&](uint32_t id) { return id >= lo && id < hi; };
-    const bool empty = sh.some == 0;
     const bool masked = kForward && c.tail;
     float *state = c.state ? c.state + row * 4 : nullptr;
+    bool arrived = true;
+    if (kResident && copied) {
+        arrived = mbar_wait(&bar, 0);
+        if (!arrived) arrived = mbar_wait(&bar, 0);
+    }
+    __syncthreads();
+    const bool unordered = sh.unordered != 0;
 
     // The entries' student logits, before anything is written (the gradient
     // may replace the logits).
-    __syncthreads();
-    for (uint32_t k = threadIdx.x; k < n; k += kThreads)
-        sh.v[k] = here(sh.id[k]) ? __fmul_rn(elem_to_float<T>(x[sh.id[k]]), c.scale) : kNegInf;
+    if (!empty)
+        for (uint32_t k = threadIdx.x; k < n; k += kThreads)
+            e.v[k] = here(e.id[k]) ? __fmul_rn(elem_to_float<T>(src[e.id[k]]), c.scale) : kNegInf;
 
     if (kForward && !empty) {
-        // Bit b stands for element body - pad + b, so that a word's elements
-        // start at a multiple of kE.
-        const uint32_t pad = (32u - ((seg.body - lo) & 31u)) & 31u;
-        if (masked) {
-            for (uint32_t w = threadIdx.x; w < (hi - lo + pad + 31u) / 32u; w += kThreads) bits[w] = 0;
+        if (kResident && masked) {
             __syncthreads();
             for (uint32_t k = threadIdx.x; k < n; k += kThreads)
-                if (here(sh.id[k])) {
-                    const uint32_t b = sh.id[k] - lo + pad;
-                    atomicOr(&bits[b / 32u], 1u << (b % 32u));
-                }
+                if (here(e.id[k])) held[e.id[k]] = from_float<T>(kNegInf);
         }
         __syncthreads();
         float m = kNegInf;
-        double s = 0.0;
-        auto one = [&](uint32_t j) {
-            const uint32_t b = j - lo + pad;
-            if (masked && (bits[b / 32u] >> (b % 32u) & 1u)) return;
-            const float v = __fmul_rn(elem_to_float<T>(x[j]), c.scale);
-            sum_batch<1>(m, s, &v);
-        };
-        if (threadIdx.x < seg.body - lo) one(lo + threadIdx.x);
-        if (threadIdx.x >= 32 && threadIdx.x - 32 < hi - seg.tail) one(seg.tail + threadIdx.x - 32);
-        const uint4 *words = reinterpret_cast<const uint4 *>(x + seg.body);
-        for (uint32_t q0 = threadIdx.x; q0 < seg.n_vec; q0 += kThreads * kLoads) {
-            uint4 w[kLoads];
-#pragma unroll
-            for (uint32_t k = 0; k < kLoads; ++k) {
-                const uint32_t q = q0 + k * kThreads;
-                w[k] = q < seg.n_vec ? words[q] : make_uint4(0, 0, 0, 0);
-            }
-            float v[kLoads * kE];
-#pragma unroll
-            for (uint32_t k = 0; k < kLoads; ++k) {
-                const uint32_t q = q0 + k * kThreads;
-                unpack<T>(w[k], v + k * kE);
-#pragma unroll
-                for (uint32_t i = 0; i < kE; ++i)
-                    v[k * kE + i] = q < seg.n_vec ? __fmul_rn(v[k * kE + i], c.scale) : kNegInf;
-                if (masked && q < seg.n_vec) {
-                    const uint32_t b = seg.body - lo + pad + q * kE;
-                    const uint32_t set = bits[b / 32u] >> (b % 32u) & ((1u << kE) - 1u);
-                    if (set) {
-#pragma unroll
-                        for (uint32_t i = 0; i < kE; ++i)
-                            if (set >> i & 1u) v[k * kE + i] = kNegInf;
-                    }
-                }
-            }
-#pragma unroll
-            for (uint32_t k = 0; k < kLoads * kE; k += 16) sum_batch<16>(m, s, v + k);
-        }
-        sum_join_lanes(m, s, 32);
+        double sum = 0.0;
+        if (kResident)
+            sum_resident<T>(c, src, seg, m, sum);
+        else
+            sum_streamed<T>(c, x, seg, reinterpret_cast<uint32_t *>(dynamic), e, n, m, sum);
+        // A copy that never came (its wait is bounded): the row reports NaN.
+        if (!arrived) sum = __longlong_as_double(0x7ff8000000000000ll);
+        float s = static_cast<float>(sum);
+        join_lanes(m, s);
         if (lane == 0) {
             sh.red_m[warp] = m;
             sh.red_s[warp] = s;
         }
+        // With the tail, the listed tokens' own sum, each id once.
+        const uint32_t warps = list_warps(n);
+        if (masked && warp < warps) {
+            float ml = kNegInf, sl = 0.0f;
+            for (uint32_t k = threadIdx.x; k < n; k += kThreads) ml = fmaxf(ml, e.v[k]);
+            ml = warp_top(ml);
+            for (uint32_t k = threadIdx.x; k < n; k += kThreads) {
+                float t_sum;
+                if (here(e.id[k]) && e.v[k] != kNegInf && first_of_id(e, unordered, n, k, t_sum))
+                    sl = __fadd_rn(sl, exp_fast(__fsub_rn(e.v[k], ml)));
+            }
+            sl = warp_sum(sl);
+            if (lane == 0) {
+                sh.list_m[warp] = ml;
+                sh.list_s[warp] = sl;
+            }
+        }
         __syncthreads();
         cluster.barrier_wait();
+        // The CTA's share to its peers (the loss alone is made by the first).
+        const bool to_peer = lane < (kGrad ? ctas : 1u);
         if (warp == 0) {
             m = lane < kWarps ? sh.red_m[lane] : kNegInf;
-            s = lane < kWarps ? sh.red_s[lane] : 0.0;
-            sum_join_lanes(m, s, kWarps);
-            // The entries of this segment: their part of the loss, and with the
-            // tail their own sum, each id once.
-            float ml = kNegInf;
-            double sl = 0.0, cross = 0.0, held = 0.0;
-            for (uint32_t k = lane; k < n; k += 32) {
-                if (!here(sh.id[k])) continue;
-                const double v = sh.v[k];
-                float t_sum;
-                if (masked && first_of_id(sh, n, k, t_sum)) sum_join(ml, sl, sh.v[k], sh.v[k] == kNegInf ? 0.0 : 1.0);
-                if (sh.t[k] == 0.0f) continue;
-                cross += static_cast<double>(sh.t[k]) * (static_cast<double>(sh.y[k]) - sh.log_norm - v);
-                held += static_cast<double>(sh.t[k]);
+            s = lane < kWarps ? sh.red_s[lane] : 0.0f;
+            join_lanes(m, s);
+            float ml = kNegInf, sl = 0.0f;
+            if (masked) {
+                ml = lane < warps ? sh.list_m[lane] : kNegInf;
+                sl = lane < warps ? sh.list_s[lane] : 0.0f;
+                join_lanes(ml, sl);
             }
-            sum_join_lanes(ml, sl, 32);
-            cross = warp_sum(cross);
-            held = warp_sum(held);
-            if (lane < ctas) {
+            if (to_peer) {
                 RowShare &to = cluster.map_shared_rank(&sh, lane)->share[rank];
                 to.max_rest = m;
                 to.sum_rest = s;
                 to.max_listed = ml;
                 to.sum_listed = sl;
+            }
+        } else if (warp == 1) {
+            // Its entries' part of the loss.
+            double cross = 0.0, held_t = 0.0;
+            for (uint32_t k = lane; k < n; k += 32) {
+                const double t = e.t[k];
+                if (!here(e.id[k]) || t == 0.0) continue;
+                cross += t * (static_cast<double>(e.y[k]) - static_cast<double>(te.y_ref) -
+                              static_cast<double>(e.v[k]));
+                held_t += t;
+            }
+            cross = warp_sum(cross);
+            held_t = warp_sum(held_t);
+            if (lane == 0) {
+                RowShare &to = cluster.map_shared_rank(&sh, 0)->share[rank];
                 to.cross = cross;
-                to.held = held;
+                to.held = held_t;
             }
         }
         cluster.sync();
-        if (threadIdx.x == 0) {
-            float mr = kNegInf, ma = kNegInf;
-            double sr = 0.0, sa = 0.0, loss = 0.0, held = 0.0;
-            for (uint32_t r = 0; r < ctas; ++r) {
-                sum_join(mr, sr, sh.share[r].max_rest, sh.share[r].sum_rest);
-                sum_join(ma, sa, sh.share[r].max_listed, sh.share[r].sum_listed);
-                loss += sh.share[r].cross;
-                held += sh.share[r].held;
+        if (warp == 0 && (kGrad || rank == 0)) {
+            const bool in = lane < ctas;
+            float mr = in ? sh.share[lane].max_rest : kNegInf;
+            float sr = in ? sh.share[lane].sum_rest : 0.0f;
+            join_lanes(mr, sr);
+            float ml = kNegInf, sl = 0.0f;
+            if (masked) {
+                ml = in ? sh.share[lane].max_listed : kNegInf;
+                sl = in ? sh.share[lane].sum_listed : 0.0f;
+                join_lanes(ml, sl);
             }
-            sum_join(ma, sa, mr, sr);
-            // A row of -inf alone has no distribution: NaN, as a NaN or +inf
-            // logit gives through the sum.
-            if (!(sa > 0.0)) sa = __longlong_as_double(0x7ff8000000000000ll);
-            const double lse = static_cast<double>(ma) + log(sa);
-            loss += held * lse;
-            // The unlisted tokens' factor against their own maximum. Without any
-            // mass there (mr = -inf) it is 0.
-            double factor = 0.0;
-            if (sr != 0.0)
-                factor = sh.mass * exp(static_cast<double>(mr) - static_cast<double>(ma)) / sa;
-            if (sh.r > 0.0) {
-                loss += sh.r * (log(sh.r) + lse);
-                loss -= sh.r * (sr != 0.0 ? static_cast<double>(mr) + log(sr) : static_cast<double>(kNegInf));
-                if (sr != 0.0) factor -= sh.r / sr;
+            const float row_max = fmaxf(mr, ml);
+            float all = __fadd_rn(mr == kNegInf ? sr : __fmul_rn(sr, exp_fast(__fsub_rn(mr, row_max))),
+                                  ml == kNegInf ? sl : __fmul_rn(sl, exp_fast(__fsub_rn(ml, row_max))));
+            // A row of -inf alone has no distribution: NaN, as a NaN or +inf logit
+            // gives through the sum.
+            if (!(all > 0.0f)) all = __uint_as_float(0x7fc00000u);
+            const float inv = __fdiv_rn(1.0f, all);
+            // The unlisted tokens' factor against their own maximum. Without any mass
+            // there (mr = -inf) it is 0.
+            const float rest_max = mr == kNegInf ? 0.0f : mr;
+            float factor = 0.0f;
+            if (sr != 0.0f) {
+                factor = __fmul_rn(__fmul_rn(static_cast<float>(te.mass), exp_fast(__fsub_rn(mr, row_max))), inv);
+                if (te.r > 0.0) factor = __fsub_rn(factor, __fdiv_rn(static_cast<float>(te.r), sr));
             }
-            sh.max = ma;
-            sh.inv = static_cast<float>(1.0 / sa);
-            sh.rest_max = mr == kNegInf ? 0.0f : mr;
-            sh.rest_factor = static_cast<float>(sa == sa ? factor : sa);
-            if (rank == 0) {
-                c.loss[row] = static_cast<float>(loss);
-                if (state) {
-                    state[0] = sh.max;
-                    state[1] = sh.inv;
-                    state[2] = sh.rest_max;
-                    state[3] = sh.rest_factor;
+            factor = __fmul_rn(factor, static_cast<float>(ExpRef(c, rest_max).correction(c)));
+            if (!(all == all)) factor = all;
+            if (lane == 0) {
+                sh.row = make_float4(row_max, inv, rest_max, factor);
+                if (rank == 0 && state) *reinterpret_cast<float4 *>(state) = sh.row;
+                sh.red_m[0] = mr;
+                sh.red_s[0] = sr;
+                sh.red_s[1] = all;
+            }
+        }
+        __syncthreads();
+        // The loss, one warp's work while the others write the gradient.
+        if (rank == 0 && warp == kWarps - 1) {
+            double loss = warp_sum(lane < ctas ? sh.share[lane].cross : 0.0);
+            const double held_all = warp_sum(lane < ctas ? sh.share[lane].held : 0.0);
+            if (lane == 0) {
+                const float mr = sh.red_m[0], sr = sh.red_s[0];
+                const double lse = static_cast<double>(sh.row.x) + log(static_cast<double>(sh.red_s[1]));
+                loss += held_all * (c.tail ? lse : lse - log(te.sum));
+                if (te.r > 0.0) {
+                    loss += te.r * (log(te.r) + lse);
+                    loss -= te.r * (sr != 0.0f ? static_cast<double>(mr) + log(static_cast<double>(sr))
+                                               : static_cast<double>(kNegInf));
                 }
+                c.loss[row] = static_cast<float>(loss);
             }
         }
     } else if (kForward && rank == 0 && threadIdx.x == 0) {
         c.loss[row] = 0.0f;
-        if (state) state[0] = state[1] = state[2] = state[3] = 0.0f;
-    }
-    if (!kForward && threadIdx.x == 0) {
-        sh.max = state[0];
-        sh.inv = state[1];
-        sh.rest_max = state[2];
-        sh.rest_factor = state[3];
+        if (state) *reinterpret_cast<float4 *>(state) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
     if (kGrad) {
-        __syncthreads();
+        if (!kForward || empty) __syncthreads();  // every entry's logit is read
+        // The row as the gradient needs it: p = exp(v - row_max) * inv on the listed
+        // tokens, exp(v - rest_max) * rest_factor the whole term on the others.
+        const float4 st = kForward ? sh.row : *reinterpret_cast<const float4 *>(state);
+        const float row_max = st.x, inv = st.y, rest_max = empty ? 0.0f : st.z, rest_factor = st.w;
         T *g = static_cast<T *>(c.dlogits) + row * c.grad_stride;
         const float up = c.row_grads[row];
         // An empty row, or one whose loss does not count, has no gradient,
         // whatever its logits hold.
         const bool none = empty || up == 0.0f;
         const float by = __fmul_rn(up, c.scale);
-        const float rest_max = sh.rest_max;
-        const float factor = none ? 0.0f : __fmul_rn(by, sh.rest_factor);
-        auto grad = [&](float xv) {
-            return none ? 0.0f
-                        : __fmul_rn(exp_fast(__fsub_rn(__fmul_rn(xv, c.scale), rest_max)), factor);
+        const ExpRef r(c, rest_max);
+        const float factor = __fmul_rn(by, rest_factor);
+        auto one = [&](uint32_t j) {
+            g[j] = from_float<T>(
+                none ? 0.0f : __fmul_rn(exp_one(elem_to_float<T>(src[j]), c.scale, r), factor));
         };
         const Segment<T> to(g, lo, hi);
         if (to.body == seg.body) {
-            auto one = [&](uint32_t j) { g[j] = from_float<T>(grad(none ? 0.0f : elem_to_float<T>(x[j]))); };
             if (threadIdx.x < seg.body - lo) one(lo + threadIdx.x);
             if (threadIdx.x >= 32 && threadIdx.x - 32 < hi - seg.tail) one(seg.tail + threadIdx.x - 32);
-            const uint4 *words = reinterpret_cast<const uint4 *>(x + seg.body);
+            const uint4 *words = reinterpret_cast<const uint4 *>(src + seg.body);
             uint4 *out = reinterpret_cast<uint4 *>(g + seg.body);
-            for (uint32_t q0 = threadIdx.x; q0 < seg.n_vec; q0 += kThreads * kLoads) {
-                uint4 w[kLoads];
+            if (none) {
+                for (uint32_t q = threadIdx.x; q < seg.n_vec; q += kThreads) out[q] = make_uint4(0, 0, 0, 0);
+            } else if (r.wide) {
+                for (uint32_t q = threadIdx.x; q < seg.n_vec; q += kThreads)
+                    out[q] = grad_word<T, true>(words[q], c.scale, r, factor);
+            } else {
+                uint32_t q0 = threadIdx.x;
+                for (; q0 + kThreads * (kLoads - 1) < seg.n_vec; q0 += kThreads * kLoads) {
+                    uint4 w[kLoads];
 #pragma unroll
-                for (uint32_t k = 0; k < kLoads; ++k) {
-                    const uint32_t q = q0 + k * kThreads;
-                    w[k] = q < seg.n_vec && !none ? words[q] : make_uint4(0, 0, 0, 0);
+                    for (uint32_t k = 0; k < kLoads; ++k) w[k] = words[q0 + k * kThreads];
+#pragma unroll
+                    for (uint32_t k = 0; k < kLoads; ++k)
+                        out[q0 + k * kThreads] = grad_word<T, false>(w[k], c.scale, r, factor);
                 }
-#pragma unroll
-                for (uint32_t k = 0; k < kLoads; ++k) {
-                    const uint32_t q = q0 + k * kThreads;
-                    float v[kE];
-                    unpack<T>(w[k], v);
-                    union {
-                        uint4 word;
-                        T elem[kE];
-                    } o;
-#pragma unroll
-                    for (uint32_t i = 0; i < kE; ++i) o.elem[i] = from_float<T>(grad(v[i]));
-                    if (q < seg.n_vec) out[q] = o.word;
-                }
+                for (; q0 < seg.n_vec; q0 += kThreads)
+                    out[q0] = grad_word<T, false>(words[q0], c.scale, r, factor);
             }
         } else {
             // The gradient's rows start at another 16-byte phase than the logits'.
-            for (uint32_t j = lo + threadIdx.x; j < hi; j += kThreads)
-                g[j] = from_float<T>(grad(none ? 0.0f : elem_to_float<T>(x[j])));
+            for (uint32_t j = lo + threadIdx.x; j < hi; j += kThreads) one(j);
         }
         // The listed tokens' gradients replace what the loop wrote there.
         __syncthreads();
         if (!none) {
-            const float mass = static_cast<float>(sh.mass);
+            const float mass = static_cast<float>(te.mass);
             for (uint32_t k = threadIdx.x; k < n; k += kThreads) {
                 float t_sum;
-                if (!here(sh.id[k]) || !first_of_id(sh, n, k, t_sum)) continue;
-                const float p = __fmul_rn(exp_fast(__fsub_rn(sh.v[k], sh.max)), sh.inv);
-                g[sh.id[k]] = from_float<T>(__fmul_rn(by, __fsub_rn(__fmul_rn(p, mass), t_sum)));
+                if (!here(e.id[k]) || !first_of_id(e, unordered, n, k, t_sum)) continue;
+                const float p = __fmul_rn(exp_fast(__fsub_rn(e.v[k], row_max)), inv);
+                g[e.id[k]] = from_float<T>(__fmul_rn(by, __fsub_rn(__fmul_rn(p, mass), t_sum)));
             }
         }
     }
-    // A CTA's shared memory outlives its peers' writes to it.
-    if (kForward && !empty) cluster.sync();
 }
 
-template <typename T, bool kForward, bool kGrad>
-cudaError_t launch(const DistillCall &c, uint32_t ctas, cudaStream_t stream) {
-    const uint32_t seg = ((c.vocab + ctas - 1) / ctas + 31u) & ~31u;
-    const size_t smem = kForward && c.tail ? (seg / 32u + 2u) * sizeof(uint32_t) : 0;
-    auto kernel = distill_kernel<T, kForward, kGrad>;
-    if (smem > (24u << 10)) {  // above the default limit, together with the static part
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             static_cast<int>(smem));
-        if (e != cudaSuccess) return e;
-    }
+// Largest segment of the resident kernel (with its phase): one CTA an SM.
+constexpr size_t kResidentMax = 200u << 10;
+
+template <typename T, bool kForward, bool kGrad, bool kResident>
+cudaError_t launch(const DistillCall &c, uint32_t ctas, size_t buffer, cudaStream_t stream) {
+    buffer = (buffer + 15u) & ~size_t{15};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(c.rows * ctas, 1, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
-    cfg.dynamicSmemBytes = smem;
+    cfg.dynamicSmemBytes = buffer + c.cap * kEntryBytes;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -412,32 +763,67 @@ cudaError_t launch(const DistillCall &c, uint32_t ctas, cudaStream_t stream) {
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, c, ctas);
+    return cudaLaunchKernelEx(&cfg, distill_kernel<T, kForward, kGrad, kResident>, c, ctas,
+                              static_cast<uint32_t>(buffer));
 }
 
 template <typename T>
-cudaError_t launch_typed(const DistillCall &c, bool forward, bool grad, uint32_t ctas,
+cudaError_t launch_typed(const DistillCall &c, bool forward, bool grad, int num_sms,
                          cudaStream_t stream) {
-    if (forward)
-        return grad ? launch<T, true, true>(c, ctas, stream) : launch<T, true, false>(c, ctas, stream);
-    return launch<T, false, true>(c, ctas, stream);
-}
-
-}  // namespace
-
-cudaError_t launch_distill(const DistillCall &c, rsc_dtype dtype, bool forward, bool grad, int num_sms,
-                           cudaStream_t stream) {
     // Four CTAs per SM, in segments of at least 2048 logits.
     uint32_t ctas = 1;
     while (ctas < kMaxCtas && static_cast<size_t>(c.rows) * ctas < 4u * static_cast<size_t>(num_sms) &&
            c.vocab / (ctas * 2) >= 2048)
         ctas *= 2;
+    if (!forward) return launch<T, false, true, false>(c, ctas, 0, stream);
+    const auto seg_of = [&](uint32_t n) { return ((c.vocab + n - 1) / n + 31u) & ~31u; };
+    // Segments of at most 52 KB: four CTAs of an SM, some copying while others
+    // compute and write.
+    const size_t bytes = static_cast<size_t>(c.vocab) * sizeof(T), share = 52u << 10;
+    const uint32_t want = static_cast<uint32_t>(std::min<size_t>(kMaxCtas, (bytes + share - 1) / share));
+    const uint32_t resident = std::max(ctas, want);
+    const size_t smem = seg_of(resident) * sizeof(T) + 16;
+    if (grad && smem <= kResidentMax) return launch<T, true, true, true>(c, resident, smem, stream);
+    // The loss alone is streamed; wider rows are too, twice for their gradient.
     // The bitmap of a segment fits in shared memory.
     while (ctas < kMaxCtas && c.vocab / ctas > (1u << 20)) ctas *= 2;
+    const size_t bits = c.tail ? (seg_of(ctas) / 32u + 2u) * sizeof(uint32_t) : 0;
+    return grad ? launch<T, true, true, false>(c, ctas, bits, stream)
+                : launch<T, true, false, false>(c, ctas, bits, stream);
+}
+
+template <typename T>
+cudaError_t setup_typed() {
+    const int most = static_cast<int>(kResidentMax + kDistillMaxTop * kEntryBytes);
+    cudaError_t e = cudaFuncSetAttribute(distill_kernel<T, true, true, true>,
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(distill_kernel<T, true, true, false>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(distill_kernel<T, true, false, false>,
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+    return e;
+}
+
+}  // namespace
+
+cudaError_t distill_setup() {
+    cudaError_t e = setup_typed<float>();
+    if (e == cudaSuccess) e = setup_typed<__nv_bfloat16>();
+    if (e == cudaSuccess) e = setup_typed<__half>();
+    return e;
+}
+
+cudaError_t launch_distill(const DistillCall &call, rsc_dtype dtype, bool forward, bool grad, int num_sms,
+                           cudaStream_t stream) {
+    DistillCall c = call;
+    c.exp2_scale = c.scale * 1.44269504f;
+    c.exp2_ratio = static_cast<double>(c.exp2_scale) / static_cast<double>(c.scale);
     switch (dtype) {
-        case RSC_F32: return launch_typed<float>(c, forward, grad, ctas, stream);
-        case RSC_BF16: return launch_typed<__nv_bfloat16>(c, forward, grad, ctas, stream);
-        case RSC_F16: return launch_typed<__half>(c, forward, grad, ctas, stream);
+        case RSC_F32: return launch_typed<float>(c, forward, grad, num_sms, stream);
+        case RSC_BF16: return launch_typed<__nv_bfloat16>(c, forward, grad, num_sms, stream);
+        case RSC_F16: return launch_typed<__half>(c, forward, grad, num_sms, stream);
     }
     return cudaErrorInvalidValue;
 }

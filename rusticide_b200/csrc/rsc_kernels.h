@@ -237,6 +237,8 @@ struct VerifyCall {
     int32_t *out_status;                  // [n_seqs]
 };
 
+// Lets the draw kernel take clusters of 16 on the current device (once).
+cudaError_t verify_setup();
 size_t verify_workspace_bytes(size_t n_seqs, size_t max_drafts, size_t vocab);
 // Two launches (rows, then decisions and draws); *launches counts them.
 // vocab > 0, n_seqs > 0.
@@ -253,6 +255,8 @@ struct DistillCall {
     uint32_t rows, vocab;
     float scale;
     int tail;
+    float exp2_scale;   // scale * log2(e), and their quotient (set by launch_distill)
+    double exp2_ratio;
     const void *logits;
     size_t row_stride;
     size_t cap;             // teacher slots per row, at most kDistillMaxTop
@@ -266,6 +270,8 @@ struct DistillCall {
     float *state;           // [rows][4]: maximum, 1 / sum, unlisted maximum, unlisted factor; nullable in forward
 };
 
+// Lets the kernels take their shared memory on the current device (once).
+cudaError_t distill_setup();
 // One launch: the loss (forward), its gradient, or both. rows, vocab > 0.
 cudaError_t launch_distill(const DistillCall &c, rsc_dtype dtype, bool forward, bool grad, int num_sms,
                            cudaStream_t stream);

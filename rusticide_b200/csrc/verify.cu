@@ -1088,10 +1088,6 @@ cudaError_t launch_verify(const VerifyCall &call, bool greedy, int num_sms, uint
         return cudaLaunchKernelEx(&cfg, verify_greedy_kernel, c);
     }
     const uint32_t ctas = draw_ctas(c.n_seqs, c.vocab, num_sms);
-    if (ctas > 8) {
-        e = cudaFuncSetAttribute(verify_draw_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return e;
-    }
     cfg.gridDim = dim3(c.n_seqs * ctas, 1, 1);
     cfg.blockDim = dim3(kDrawThreads, 1, 1);
     cfg.dynamicSmemBytes = sizeof(DrawShared);
@@ -1106,6 +1102,10 @@ cudaError_t launch_verify(const VerifyCall &call, bool greedy, int num_sms, uint
         cfg.numAttrs = 1;
     }
     return cudaLaunchKernelEx(&cfg, verify_draw_kernel, c, ctas);
+}
+
+cudaError_t verify_setup() {
+    return cudaFuncSetAttribute(verify_draw_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
 }
 
 cudaError_t launch_verify_records(const VerifyCall &c, cudaStream_t stream) {

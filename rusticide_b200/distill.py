@@ -19,12 +19,9 @@ from .sampler import engine
 class _DistillLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, logprobs, n, temperature, tail):
-        want = ctx.needs_input_grad[0]
-        loss, state = engine(logits.device).distill_forward(
-            logits, ids, logprobs, n, temperature, tail, want_state=want)
-        if want:
-            ctx.save_for_backward(logits, ids, logprobs, n, state)
-            ctx.how = (temperature, tail)
+        loss, state = engine(logits.device).distill_forward(logits, ids, logprobs, n, temperature, tail)
+        ctx.save_for_backward(logits, ids, logprobs, n, state)
+        ctx.how = (temperature, tail)
         return loss
 
     @staticmethod
@@ -44,4 +41,7 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor
     header), n [...] int32 of them a row. Returns [...] f32; differentiable once, with respect to
     the logits. A training loop that knows each row's weight beforehand takes
     `Engine.distill_step`, which gives loss and gradient in one pass."""
-    return _DistillLoss.apply(logits, ids, logprobs, n, float(temperature), bool(tail))
+    if logits.requires_grad and torch.is_grad_enabled():
+        return _DistillLoss.apply(logits, ids, logprobs, n, temperature, tail)
+    return engine(logits.device).distill_forward(logits, ids, logprobs, n, temperature, tail,
+                                                 want_state=False)[0]

@@ -396,17 +396,17 @@ class Engine:
         return ids, status, probs
 
     # -- verification of drafted tokens ---------------------------------------
-    def _want(self, t: torch.Tensor, what: str, dtype: torch.dtype, shape: tuple) -> int:
+    def _want(self, t: torch.Tensor, what: str, dtype: torch.dtype, shape) -> int:
         """The address of a dense argument of this type and shape on the engine's device."""
+        if t.dtype is dtype and t.shape == shape and t.device == self.device and t.is_contiguous():
+            return t.data_ptr()
         if t.device != self.device:
             raise ValueError(f"{what} on {t.device}, engine on {self.device}")
         if t.dtype != dtype:
             raise TensorError(str(dtype).replace("torch.", ""), str(t.dtype).replace("torch.", ""))
         if t.shape != shape:
             raise InvalidShape(list(t.shape))
-        if not t.is_contiguous():
-            raise ValueError(f"{what} must be contiguous")
-        return t.data_ptr()
+        raise ValueError(f"{what} must be contiguous")
 
     def _rows_3d(self, t: torch.Tensor, what: str, shape: tuple) -> tuple[int, int, int]:
         """(address, sequence stride, row stride) of [sequences, rows, vocab] f32 logits whose rows
@@ -419,7 +419,7 @@ class Engine:
             raise InvalidShape(list(t.shape))
         seqs, rows, vocab = shape
         ss, rs, es = t.stride()
-        if vocab > 1 and es != 1 and t.numel() > 0:
+        if es != 1 and vocab > 1 and t.numel() > 0:
             raise ValueError("logit rows must be contiguous")
         # A dimension of one element has no stride to go by.
         rs = rs if rows > 1 else vocab
@@ -429,21 +429,17 @@ class Engine:
         if draft_tokens.dim() != 2:
             raise InvalidShape(list(draft_tokens.shape))
         seqs, drafts = draft_tokens.shape
-        x = _lib.RscDraftBatch()
-        x.n_seqs, x.max_drafts = seqs, drafts
-        x.d_draft_tokens = self._want(draft_tokens, "draft_tokens", torch.int32, (seqs, drafts))
-        if n_draft is not None:
-            x.d_n_draft = self._want(n_draft, "n_draft", torch.int32, (seqs,))
+        tokens = self._want(draft_tokens, "draft_tokens", torch.int32, (seqs, drafts))
+        counts = None if n_draft is None else self._want(n_draft, "n_draft", torch.int32, (seqs,))
+        vocab, target, draft = 0, (None, 0, 0), (None, 0, 0)
         if target_logits is not None:
             if target_logits.dim() != 3:
                 raise InvalidShape(list(target_logits.shape))
-            x.vocab = vocab = target_logits.shape[2]
-            x.d_target, x.target_seq_stride, x.target_row_stride = self._rows_3d(
-                target_logits, "target_logits", (seqs, drafts + 1, vocab))
+            vocab = target_logits.shape[2]
+            target = self._rows_3d(target_logits, "target_logits", (seqs, drafts + 1, vocab))
             if draft_logits is not None and drafts > 0:
-                x.d_draft, x.draft_seq_stride, x.draft_row_stride = self._rows_3d(
-                    draft_logits, "draft_logits", (seqs, drafts, vocab))
-        return x
+                draft = self._rows_3d(draft_logits, "draft_logits", (seqs, drafts, vocab))
+        return _lib.RscDraftBatch(seqs, drafts, vocab, *target, *draft, tokens, counts)
 
     def _verify_draws(self, seqs: int, drafts: int, uniforms, rng_states):
         u = None if uniforms is None else self._want(uniforms, "uniforms", torch.float32,
@@ -451,12 +447,11 @@ class Engine:
         st = None if rng_states is None else self._want(rng_states, "rng_states", torch.int64, (seqs,))
         return u, st
 
-    def _verify_outputs(self, seqs: int, drafts: int, out):
+    def _verify_outputs(self, draft_tokens: torch.Tensor, out):
+        seqs, drafts = draft_tokens.shape
         if out is None:
-            dev = self.device
-            return (torch.empty((seqs, drafts + 1), dtype=torch.int32, device=dev),
-                    torch.empty(seqs, dtype=torch.int32, device=dev),
-                    torch.empty(seqs, dtype=torch.int32, device=dev))
+            return (draft_tokens.new_empty((seqs, drafts + 1)), draft_tokens.new_empty(seqs),
+                    draft_tokens.new_empty(seqs))
         for t, what, shape in zip(out, ("tokens", "accepted", "status"),
                                   ((seqs, drafts + 1), (seqs,), (seqs,))):
             self._want(t, f"out {what}", torch.int32, shape)
@@ -496,9 +491,9 @@ class Engine:
             return self.verify_survivors(target, draft_tokens, uniforms=uniforms,
                                          rng_states=rng_states, draft=draft, n_draft=n_draft, out=out)
         u, st = self._verify_draws(seqs, drafts, uniforms, rng_states)
-        tokens, accepted, status = self._verify_outputs(seqs, drafts, out)
+        tokens, accepted, status = self._verify_outputs(draft_tokens, out)
         nbytes = self.lib.rsc_verify_workspace_bytes(seqs, drafts, vocab)
-        work = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        work = draft_tokens.new_empty(nbytes // 4)
         check(self.lib.rsc_verify(self._h, ctypes.byref(x), ctypes.byref(params.to_c()), u, st,
                                   work.data_ptr(), nbytes, tokens.data_ptr(), accepted.data_ptr(),
                                   status.data_ptr(), _stream_ptr(self.device)), "rsc_verify")
@@ -547,7 +542,7 @@ class Engine:
         d = None
         if draft is not None and drafts > 0:
             d = ctypes.byref(self._record_struct(draft, "draft", seqs * drafts))
-        tokens, accepted, status = self._verify_outputs(seqs, drafts, out)
+        tokens, accepted, status = self._verify_outputs(draft_tokens, out)
         check(self.lib.rsc_verify_survivors(self._h, ctypes.byref(x), ctypes.byref(t), d, u, st,
                                             tokens.data_ptr(), accepted.data_ptr(),
                                             status.data_ptr(), _stream_ptr(self.device)),
@@ -566,22 +561,20 @@ class Engine:
             raise TensorError("f32, bf16 or f16", str(logits.dtype).replace("torch.", ""))
         if logits.dim() < 1 or ids.shape[:-1] != logits.shape[:-1] or ids.dim() != logits.dim():
             raise InvalidShape(list(ids.shape))
-        lead, vocab, cap = logits.shape[:-1], logits.shape[-1], ids.shape[-1]
-        rows = 1
-        for k in lead:
-            rows *= k
-        x = logits if logits.dim() == 2 else logits.reshape(rows, vocab)
-        if rows > 0 and vocab > 1 and (x.stride(1) != 1 or (rows > 1 and x.stride(0) < vocab)):
+        shape = logits.shape
+        lead, vocab, cap = shape[:-1], shape[-1], ids.shape[-1]
+        rows = lead.numel()
+        x = logits if len(shape) == 2 else logits.reshape(rows, vocab)
+        stride, step = x.stride()
+        if rows > 0 and vocab > 1 and (step != 1 or (rows > 1 and stride < vocab)):
             x = x.contiguous()  # rows out of order, or one row broadcast to many
-        b = _lib.RscDistillBatch()
-        b.rows, b.vocab, b.dtype, b.tail, b.temperature, b.cap = (
-            rows, vocab, dtype, bool(tail), float(temperature), cap)
-        b.d_logits, b.row_stride = x.data_ptr(), x.stride(0) if rows > 1 else vocab
-        b.d_ids = self._want(ids, "ids", torch.int32, (*lead, cap))
-        b.d_logprobs = self._want(logprobs, "logprobs", torch.float32, (*lead, cap))
-        if n is not None:
-            b.d_n = self._want(n, "n", torch.int32, lead)
-        return b, x
+            stride = vocab
+        entries = (*lead, cap)
+        return _lib.RscDistillBatch(
+            rows, vocab, x.data_ptr(), stride if rows > 1 else vocab, dtype, bool(tail), temperature,
+            cap, None if n is None else self._want(n, "n", torch.int32, lead),
+            self._want(ids, "ids", torch.int32, entries),
+            self._want(logprobs, "logprobs", torch.float32, entries)), x
 
     def distill_forward(self, logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor,
                         n: Optional[torch.Tensor] = None, temperature: float = 1.0,
@@ -591,8 +584,8 @@ class Engine:
         and logprobs [..., top] f32, n [...] int32 of them (None: all; ids of -1 are skipped), and
         the state that distill_backward takes (None without want_state)."""
         b, x = self._distill_batch(logits, ids, logprobs, n, temperature, tail)
-        loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=self.device)
-        state = torch.empty((b.rows, 4), dtype=torch.float32, device=self.device) if want_state else None
+        loss = logprobs.new_empty(logits.shape[:-1])
+        state = logprobs.new_empty((b.rows, 4)) if want_state else None
         check(self.lib.rsc_distill(self._h, ctypes.byref(b), loss.data_ptr(), _ptr(state), None, None,
                                    0, _stream_ptr(self.device)), "rsc_distill")
         return loss, state
@@ -618,7 +611,7 @@ class Engine:
                 raise ValueError("logits of this layout cannot be replaced by their gradient")
             else:
                 stride = b.row_stride
-        loss = torch.empty(logits.shape[:-1], dtype=torch.float32, device=self.device)
+        loss = logprobs.new_empty(logits.shape[:-1])
         check(self.lib.rsc_distill(self._h, ctypes.byref(b), loss.data_ptr(), None, up, out.data_ptr(),
                                    stride, _stream_ptr(self.device)), "rsc_distill")
         return loss, out
