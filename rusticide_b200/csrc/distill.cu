@@ -13,12 +13,19 @@
 // second are multiples of exp(v_j - m), m the largest unlisted v: one
 // exponential a token, and none that vanishes where the tail's share does.
 //
-// A row is spread over a cluster of CTAs that join their sums through
-// distributed shared memory. S_tail is summed over the unlisted tokens as such
-// (a bitmap of the listed ones masks them out): S minus the listed terms would
-// lose it where the listed tokens hold nearly all of the mass. Sums leave a
-// thread's batch of 16 in binary64 (rsc_rowsum.cuh), what is computed per row
-// or per entry is binary64 throughout.
+// A row is cut into segments for a cluster of CTAs that join their sums through
+// distributed shared memory. The pass is bound by HBM (the loss alone: one
+// read), next by the exponentials (one MUFU operation each, 16 a cycle and SM)
+// and the instructions around them, so exponents and sums are taken two at a
+// time (f32x2) and a 16-byte word's maximum on its packed halves; the lists'
+// binary64 work runs while the cluster's CTAs wait for one another. S_tail is
+// summed over the unlisted tokens as such (a bitmap of the listed ones masks
+// them out): S minus the listed terms would lose it where the listed tokens
+// hold nearly all of the mass. Measured (B200, GPU time): loss of 4096 x 128256
+// bf16 with 128 entries and the tail 199 us (5.3 TB/s), loss and gradient of 2048
+// x 151936 bf16 259 us (4.8 TB/s of one read and one write). Keeping the segment
+// in shared memory between the passes (TMA copies, four CTAs of 52 KB an SM)
+// took 305-322 us: the phases of so few CTAs do not overlap.
 #include <algorithm>
 #include <type_traits>
 
@@ -68,10 +75,9 @@ constexpr size_t kEntryBytes = 16;
 
 // What is known of a row's list as a whole, in every thread.
 struct Teacher {
-    uint32_t n;
-    bool some;         // it has an entry
-    float y_ref;       // what exponents were taken against
-    double sum;        // of exp(y - y_ref)
+    bool some;     // it has an entry
+    float y_ref;   // what exponents were taken against
+    double sum;    // of exp(y - y_ref)
     double r, mass;
 };
 
@@ -123,14 +129,14 @@ __device__ __forceinline__ uint64_t pair_of(float a, float b) {
     return p;
 }
 __device__ __forceinline__ float low_of(uint64_t p) {
-    float a, b;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
+    float a;
+    asm("mov.b64 {%0, _}, %1;" : "=f"(a) : "l"(p));
     return a;
 }
 __device__ __forceinline__ float high_of(uint64_t p) {
-    float a, b;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p));
-    return b;
+    float a;
+    asm("mov.b64 {_, %0}, %1;" : "=f"(a) : "l"(p));
+    return a;
 }
 // The largest of a warp's values (NaN passed over), in every lane.
 __device__ __forceinline__ float warp_top(float v) {
@@ -212,56 +218,61 @@ __device__ __forceinline__ uint4 grad_word(const uint4 &w, float scale, const Ex
 // The id of an absent entry: one outside the vocabulary, or of no probability.
 constexpr uint32_t kAbsent = 0xffffffffu;
 
-// The teacher's list of a row, one entry a thread for lists of up to a block.
-// The exponentials are binary64: with the tail, r is what they leave of 1.
-__device__ __forceinline__ Teacher load_teacher(const DistillCall &c, size_t row, const Entries &e,
-                                                DistillShared &sh) {
-    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-    Teacher te;
-    te.n = static_cast<uint32_t>(c.cap);
-    if (c.n) te.n = min(te.n, c.n[row]);
-    const uint32_t n = te.n, warps = list_warps(n);
-    if (threadIdx.x == 0) sh.unordered = 0;
-    float top = kNegInf;
-    bool some = false, unordered = false;
+// The ids and log-probabilities of a row's list (one entry a thread for lists of
+// up to a block), absent ones marked.
+__device__ __forceinline__ void load_entries(const DistillCall &c, size_t row, uint32_t n,
+                                             const Entries &e, DistillShared &sh) {
+    const uint32_t *ids = c.ids + row * c.cap;
+    bool unordered = false;
     for (uint32_t k = threadIdx.x; k < n; k += kThreads) {
-        const uint32_t *ids = c.ids + row * c.cap;
         const uint32_t id = ids[k], next = k + 1 < n ? ids[k + 1] : kAbsent;
         const float y = c.logprobs[row * c.cap + k];
-        const bool there = id < c.vocab && y != kNegInf;
-        e.id[k] = there ? id : kAbsent;
+        e.id[k] = id < c.vocab && y != kNegInf ? id : kAbsent;
         e.y[k] = y;
         // Lists in ascending order (padding aside) hold no id twice.
         unordered |= !(id < next) && next < c.vocab;
-        some |= there;
-        if (there) top = fmaxf(top, y);
     }
-    te.some = __syncthreads_or(some);
     if (unordered) sh.unordered = 1;
+}
+
+// The entries' probabilities, from what this thread loaded. The exponentials
+// are binary64: with the tail, r is what they leave of 1. Called by the whole
+// block; it has passed a barrier before e.t is read by others.
+__device__ __forceinline__ Teacher weigh_entries(const DistillCall &c, uint32_t n, const Entries &e,
+                                                 DistillShared &sh) {
+    const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
+    const uint32_t warps = list_warps(n);
+    Teacher te;
     // With the tail the values are log-probabilities as such.
     te.y_ref = 0.0f;
+    bool some = false;
     if (!c.tail) {
         if (warp < warps) {
+            float top = kNegInf;
+            for (uint32_t k = threadIdx.x; k < n; k += kThreads)
+                if (e.id[k] != kAbsent) top = fmaxf(top, e.y[k]);
             top = warp_top(top);
             if (lane == 0) sh.red_y[warp] = top;
         }
         __syncthreads();
-        top = sh.red_y[0];
-        for (uint32_t w = 1; w < warps; ++w) top = fmaxf(top, sh.red_y[w]);
+        float top = kNegInf;
+        for (uint32_t w = 0; w < warps; ++w) top = fmaxf(top, sh.red_y[w]);
         if (fabsf(top) < kPosInf) te.y_ref = top;
     }
     if (warp < warps) {
         double part = 0.0;
         for (uint32_t k = threadIdx.x; k < n; k += kThreads) {
-            const double p = e.id[k] != kAbsent
-                                 ? exp(static_cast<double>(e.y[k]) - static_cast<double>(te.y_ref)) : 0.0;
+            const bool there = e.id[k] != kAbsent;
+            const double p =
+                there ? exp(static_cast<double>(e.y[k]) - static_cast<double>(te.y_ref)) : 0.0;
             e.t[k] = static_cast<float>(p);
             part += p;
+            some |= there;
         }
         part = warp_sum(part);
         if (lane == 0) sh.red_t[warp] = part;
     }
-    __syncthreads();
+    te.some = __syncthreads_or(some);
     te.sum = 0.0;
     for (uint32_t w = 0; w < warps; ++w) te.sum += sh.red_t[w];
     te.r = 0.0;
@@ -276,22 +287,20 @@ __device__ __forceinline__ Teacher load_teacher(const DistillCall &c, size_t row
     return te;
 }
 
-// Entry k is the first of its id, and the sum of t over the entries of that
-// id in list order (ids may repeat: each entry counts).
-__device__ __forceinline__ bool first_of_id(const Entries &e, bool unordered, uint32_t n, uint32_t k,
-                                            float &t_sum) {
-    t_sum = e.t[k];
-    if (!unordered) return true;
-    const uint32_t id = e.id[k];
+// Entry k is the first of its id (ids may repeat: each entry counts).
+__device__ __forceinline__ bool first_of_id(const Entries &e, bool unordered, uint32_t k) {
+    if (unordered)
+        for (uint32_t q = 0; q < k; ++q)
+            if (e.id[q] == e.id[k]) return false;
+    return true;
+}
+
+// The sum of t over the entries of k's id, in list order.
+__device__ __forceinline__ float sum_of_id(const Entries &e, uint32_t n, uint32_t k) {
     double sum = 0.0;
-    bool first = true;
-    for (uint32_t q = 0; q < n; ++q) {
-        if (e.id[q] != id) continue;
-        first &= q >= k;
-        sum += static_cast<double>(e.t[q]);
-    }
-    t_sum = static_cast<float>(sum);
-    return first;
+    for (uint32_t q = 0; q < n; ++q)
+        if (e.id[q] == e.id[k]) sum += static_cast<double>(e.t[q]);
+    return static_cast<float>(sum);
 }
 
 // The (m, s) pairs of a warp's lanes joined in binary32, in all of them. A sum
@@ -339,48 +348,11 @@ __device__ __forceinline__ float batch_sum(const uint4 *w, uint64_t c, uint64_t 
     return __fadd_rn(low_of(e[0]), high_of(e[0]));
 }
 
-// (m, s) of this thread's share of a segment in shared memory, src[j] the
-// element j: the maximum first, then the exponentials against it.
-template <typename T>
-__device__ __forceinline__ void sum_resident(const DistillCall &c, const T *src, const Segment<T> &seg,
-                                             float &m, double &s) {
-    constexpr int kE = kVecElems<T>;
-    const uint4 *words = reinterpret_cast<const uint4 *>(src + seg.body);
-    const bool head = threadIdx.x < seg.body - seg.lo;
-    const bool tail = threadIdx.x >= 32 && threadIdx.x - 32 < seg.hi - seg.tail;
-    float top = kNegInf;
-    for (uint32_t q = threadIdx.x; q < seg.n_vec; q += kThreads) top = fmaxf(top, word_max<T>(words[q]));
-    const float one = head ? elem_to_float<T>(src[seg.lo + threadIdx.x])
-                           : tail ? elem_to_float<T>(src[seg.tail + threadIdx.x - 32]) : kNegInf;
-    top = fmaxf(top, one);
-    m = __fmul_rn(top, c.scale);
-    const ExpRef r(c, top == kNegInf ? 0.0f : m);
-    s = static_cast<double>(exp_one(one, c.scale, r));
-    if (r.wide) {
-        for (uint32_t q = threadIdx.x; q < seg.n_vec; q += kThreads) {
-            float v[kE];
-            unpack<T>(words[q], v);
-            for (int i = 0; i < kE; ++i) s += static_cast<double>(exp_one(v[i], c.scale, r));
-        }
-        return;
-    }
-    const uint64_t cc = pair_of(r.c, r.c), mc = pair_of(-r.mc, -r.mc);
-    uint32_t q0 = threadIdx.x;
-    for (; q0 + kThreads * (kLoads - 1) < seg.n_vec; q0 += kThreads * kLoads) {
-        uint4 w[kLoads];
-#pragma unroll
-        for (uint32_t k = 0; k < kLoads; ++k) w[k] = words[q0 + k * kThreads];
-        s += static_cast<double>(batch_sum<T, kLoads>(w, cc, mc));
-    }
-    for (; q0 < seg.n_vec; q0 += kThreads) s += static_cast<double>(batch_sum<T, 1>(words + q0, cc, mc));
-    s *= r.correction(c);
-}
-
 // (m, s) of this thread's share of a segment in global memory: a batch of
 // 16-byte words at a time against one running maximum. Where the tail is wanted
 // by itself the listed elements are left out by their bit.
 template <typename T>
-__device__ __forceinline__ void sum_streamed(const DistillCall &c, const T *x, const Segment<T> &seg,
+__device__ __forceinline__ void sum_segment(const DistillCall &c, const T *x, const Segment<T> &seg,
                                              uint32_t *bits, const Entries &en, uint32_t n, float &m,
                                              double &s) {
     constexpr uint32_t kE = kVecElems<T>;
@@ -476,18 +448,12 @@ __device__ __forceinline__ void sum_streamed(const DistillCall &c, const T *x, c
     m = top > kNegInf ? r.ref : kNegInf;
 }
 
-// kResident: the CTA's segment is copied to shared memory once (1-D TMA bulk
-// copies) and read there by both passes, so a row crosses HBM once for the loss
-// and once more for the gradient's write; listed elements are overwritten with
-// -inf there instead of being looked up in a bitmap.
-template <typename T, bool kForward, bool kGrad, bool kResident>
-__global__ void __launch_bounds__(kThreads)
-distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t buffer_bytes) {
-    // The first buffer_bytes: the segment, in the 16-byte phase of its global
-    // address (resident), or one bit per element of it. Then the entries.
+template <typename T, bool kForward, bool kGrad>
+__global__ void __launch_bounds__(kThreads, kForward ? 6 : 8)
+distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bitmap_bytes) {
+    // One bit per element of the segment (with the tail), then the entries.
     extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ DistillShared sh;
-    __shared__ uint64_t bar;
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t rank = cluster.block_rank();
     const size_t row = blockIdx.x / ctas;
@@ -497,74 +463,35 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bu
     const uint32_t lo = min(c.vocab, rank * seg_len), hi = min(c.vocab, lo + seg_len);
     const Segment<T> seg(x, lo, hi);
     Entries e;
-    e.id = reinterpret_cast<uint32_t *>(dynamic + buffer_bytes);
+    e.id = reinterpret_cast<uint32_t *>(dynamic + bitmap_bytes);
     e.y = reinterpret_cast<float *>(e.id + c.cap);
     e.t = e.y + c.cap;
     e.v = e.t + c.cap;
-    // src[j]: element j, from where both passes read it.
-    const T *src = x;
-    T *held = nullptr;
-    bool copied = false;
-    if (kResident) {
-        held = reinterpret_cast<T *>(dynamic + (reinterpret_cast<uintptr_t>(x + lo) & 15u)) - lo;
-        src = held;
-        // An empty list needs no logits.
-        copied = c.cap > 0 && !(c.n && c.n[row] == 0);
-        if (threadIdx.x == 0) {
-            mbar_init(&bar, 1);
-            fence_barrier_init();
-            if (copied) {
-                mbar_arrive_expect_tx(&bar, seg.n_vec * 16u);
-                constexpr uint32_t kCopy = 1024;  // 16 KiB each
-                for (uint32_t q = 0; q < seg.n_vec; q += kCopy)
-                    tma_load_1d(held + seg.body + q * kVecElems<T>, x + seg.body + q * kVecElems<T>,
-                                min(kCopy, seg.n_vec - q) * 16u, &bar);
-            }
-        }
-        if (copied) {
-            if (threadIdx.x < seg.body - lo) held[lo + threadIdx.x] = x[lo + threadIdx.x];
-            if (threadIdx.x >= 32 && threadIdx.x - 32 < hi - seg.tail)
-                held[seg.tail + threadIdx.x - 32] = x[seg.tail + threadIdx.x - 32];
-        }
-    }
-    const Teacher te = load_teacher(c, row, e, sh);
-    const uint32_t n = te.n;
-    const bool empty = !te.some;
-    // Every CTA of the cluster runs before its memory is written (the row is
-    // empty for all of them or for none).
-    if (kForward && !empty) cluster.barrier_arrive();
+    uint32_t n = static_cast<uint32_t>(c.cap);
+    if (c.n) n = min(n, c.n[row]);
+    // A row with an empty list is not looked at (for every CTA of the cluster alike).
+    const bool listed = n > 0;
+    float *state = c.state ? c.state + row * 4 : nullptr;
+    // Every CTA of the cluster runs before its memory is written.
+    if (kForward && listed) cluster.barrier_arrive();
+    if (threadIdx.x == 0) sh.unordered = 0;
+    __syncthreads();
+    load_entries(c, row, n, e, sh);
     auto here = [&](uint32_t id) { return id >= lo && id < hi; };
     const bool masked = kForward && c.tail;
-    float *state = c.state ? c.state + row * 4 : nullptr;
-    bool arrived = true;
-    if (kResident && copied) {
-        arrived = mbar_wait(&bar, 0);
-        if (!arrived) arrived = mbar_wait(&bar, 0);
-    }
     __syncthreads();
     const bool unordered = sh.unordered != 0;
 
     // The entries' student logits, before anything is written (the gradient
     // may replace the logits).
-    if (!empty)
-        for (uint32_t k = threadIdx.x; k < n; k += kThreads)
-            e.v[k] = here(e.id[k]) ? __fmul_rn(elem_to_float<T>(src[e.id[k]]), c.scale) : kNegInf;
+    for (uint32_t k = threadIdx.x; k < n; k += kThreads)
+        e.v[k] = here(e.id[k]) ? __fmul_rn(elem_to_float<T>(x[e.id[k]]), c.scale) : kNegInf;
 
-    if (kForward && !empty) {
-        if (kResident && masked) {
-            __syncthreads();
-            for (uint32_t k = threadIdx.x; k < n; k += kThreads)
-                if (here(e.id[k])) held[e.id[k]] = from_float<T>(kNegInf);
-        }
-        __syncthreads();
+    Teacher te{};
+    if (kForward && listed) {
         float m = kNegInf;
         double sum = 0.0;
-        if (kResident)
-            sum_resident<T>(c, src, seg, m, sum);
-        else
-            sum_streamed<T>(c, x, seg, reinterpret_cast<uint32_t *>(dynamic), e, n, m, sum);
-        // A copy that never came (its wait is bounded): the row reports NaN.
-        if (!arrived) sum = __longlong_as_double(0x7ff8000000000000ll);
+        sum_segment<T>(c, x, seg, reinterpret_cast<uint32_t *>(dynamic), e, n, m, sum);
         float s = static_cast<float>(sum);
         join_lanes(m, s);
         if (lane == 0) {
@@ -577,11 +504,9 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bu
             float ml = kNegInf, sl = 0.0f;
             for (uint32_t k = threadIdx.x; k < n; k += kThreads) ml = fmaxf(ml, e.v[k]);
             ml = warp_top(ml);
-            for (uint32_t k = threadIdx.x; k < n; k += kThreads) {
-                float t_sum;
-                if (here(e.id[k]) && e.v[k] != kNegInf && first_of_id(e, unordered, n, k, t_sum))
+            for (uint32_t k = threadIdx.x; k < n; k += kThreads)
+                if (here(e.id[k]) && e.v[k] != kNegInf && first_of_id(e, unordered, k))
                     sl = __fadd_rn(sl, exp_fast(__fsub_rn(e.v[k], ml)));
-            }
             sl = warp_sum(sl);
             if (lane == 0) {
                 sh.list_m[warp] = ml;
@@ -590,8 +515,7 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bu
         }
         __syncthreads();
         cluster.barrier_wait();
-        // The CTA's share to its peers (the loss alone is made by the first).
-        const bool to_peer = lane < (kGrad ? ctas : 1u);
+        // The CTA's sums to its peers (to the first alone where the loss is all).
         if (warp == 0) {
             m = lane < kWarps ? sh.red_m[lane] : kNegInf;
             s = lane < kWarps ? sh.red_s[lane] : 0.0f;
@@ -602,15 +526,21 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bu
                 sl = lane < warps ? sh.list_s[lane] : 0.0f;
                 join_lanes(ml, sl);
             }
-            if (to_peer) {
+            if (lane < (kGrad ? ctas : 1u)) {
                 RowShare &to = cluster.map_shared_rank(&sh, lane)->share[rank];
                 to.max_rest = m;
                 to.sum_rest = s;
                 to.max_listed = ml;
                 to.sum_listed = sl;
             }
-        } else if (warp == 1) {
-            // Its entries' part of the loss.
+        }
+        // The teacher's side while the cluster's other CTAs arrive.
+        cluster.barrier_arrive();
+        te = weigh_entries(c, n, e, sh);
+        __syncthreads();
+        cluster.barrier_wait();
+        if (warp == 1) {
+            // This segment's part of the loss.
             double cross = 0.0, held_t = 0.0;
             for (uint32_t k = lane; k < n; k += 32) {
                 const double t = e.t[k];
@@ -627,7 +557,7 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bu
                 to.held = held_t;
             }
         }
-        cluster.sync();
+        cluster.barrier_arrive();
         if (warp == 0 && (kGrad || rank == 0)) {
             const bool in = lane < ctas;
             float mr = in ? sh.share[lane].max_rest : kNegInf;
@@ -658,56 +588,46 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bu
             if (!(all == all)) factor = all;
             if (lane == 0) {
                 sh.row = make_float4(row_max, inv, rest_max, factor);
-                if (rank == 0 && state) *reinterpret_cast<float4 *>(state) = sh.row;
                 sh.red_m[0] = mr;
                 sh.red_s[0] = sr;
                 sh.red_s[1] = all;
+                // (1 / sum is never 0: a state of zeros is a row without entries.)
+                if (rank == 0 && state)
+                    *reinterpret_cast<float4 *>(state) = te.some ? sh.row : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
             }
         }
         __syncthreads();
-        // The loss, one warp's work while the others write the gradient.
-        if (rank == 0 && warp == kWarps - 1) {
-            double loss = warp_sum(lane < ctas ? sh.share[lane].cross : 0.0);
-            const double held_all = warp_sum(lane < ctas ? sh.share[lane].held : 0.0);
-            if (lane == 0) {
-                const float mr = sh.red_m[0], sr = sh.red_s[0];
-                const double lse = static_cast<double>(sh.row.x) + log(static_cast<double>(sh.red_s[1]));
-                loss += held_all * (c.tail ? lse : lse - log(te.sum));
-                if (te.r > 0.0) {
-                    loss += te.r * (log(te.r) + lse);
-                    loss -= te.r * (sr != 0.0f ? static_cast<double>(mr) + log(static_cast<double>(sr))
-                                               : static_cast<double>(kNegInf));
-                }
-                c.loss[row] = static_cast<float>(loss);
-            }
-        }
     } else if (kForward && rank == 0 && threadIdx.x == 0) {
         c.loss[row] = 0.0f;
         if (state) *reinterpret_cast<float4 *>(state) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
     if (kGrad) {
-        if (!kForward || empty) __syncthreads();  // every entry's logit is read
+        if (!kForward) __syncthreads();  // every entry's logit is read
         // The row as the gradient needs it: p = exp(v - row_max) * inv on the listed
         // tokens, exp(v - rest_max) * rest_factor the whole term on the others.
-        const float4 st = kForward ? sh.row : *reinterpret_cast<const float4 *>(state);
-        const float row_max = st.x, inv = st.y, rest_max = empty ? 0.0f : st.z, rest_factor = st.w;
+        float4 st = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (!kForward)
+            st = *reinterpret_cast<const float4 *>(state);
+        else if (te.some)
+            st = sh.row;
+        const float row_max = st.x, inv = st.y, rest_max = st.z, rest_factor = st.w;
         T *g = static_cast<T *>(c.dlogits) + row * c.grad_stride;
         const float up = c.row_grads[row];
-        // An empty row, or one whose loss does not count, has no gradient,
-        // whatever its logits hold.
-        const bool none = empty || up == 0.0f;
+        // A row without an entry, or one whose loss does not count, has no
+        // gradient, whatever its logits hold.
+        const bool none = inv == 0.0f || up == 0.0f;
         const float by = __fmul_rn(up, c.scale);
         const ExpRef r(c, rest_max);
         const float factor = __fmul_rn(by, rest_factor);
         auto one = [&](uint32_t j) {
             g[j] = from_float<T>(
-                none ? 0.0f : __fmul_rn(exp_one(elem_to_float<T>(src[j]), c.scale, r), factor));
+                none ? 0.0f : __fmul_rn(exp_one(elem_to_float<T>(x[j]), c.scale, r), factor));
         };
         const Segment<T> to(g, lo, hi);
         if (to.body == seg.body) {
             if (threadIdx.x < seg.body - lo) one(lo + threadIdx.x);
             if (threadIdx.x >= 32 && threadIdx.x - 32 < hi - seg.tail) one(seg.tail + threadIdx.x - 32);
-            const uint4 *words = reinterpret_cast<const uint4 *>(src + seg.body);
+            const uint4 *words = reinterpret_cast<const uint4 *>(x + seg.body);
             uint4 *out = reinterpret_cast<uint4 *>(g + seg.body);
             if (none) {
                 for (uint32_t q = threadIdx.x; q < seg.n_vec; q += kThreads) out[q] = make_uint4(0, 0, 0, 0);
@@ -719,10 +639,10 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bu
                 for (; q0 + kThreads * (kLoads - 1) < seg.n_vec; q0 += kThreads * kLoads) {
                     uint4 w[kLoads];
 #pragma unroll
-                    for (uint32_t k = 0; k < kLoads; ++k) w[k] = words[q0 + k * kThreads];
+                    for (uint32_t k = 0; k < kLoads; ++k) w[k] = __ldcs(words + q0 + k * kThreads);
 #pragma unroll
                     for (uint32_t k = 0; k < kLoads; ++k)
-                        out[q0 + k * kThreads] = grad_word<T, false>(w[k], c.scale, r, factor);
+                        __stcs(out + q0 + k * kThreads, grad_word<T, false>(w[k], c.scale, r, factor));
                 }
                 for (; q0 < seg.n_vec; q0 += kThreads)
                     out[q0] = grad_word<T, false>(words[q0], c.scale, r, factor);
@@ -732,29 +652,45 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bu
             for (uint32_t j = lo + threadIdx.x; j < hi; j += kThreads) one(j);
         }
         // The listed tokens' gradients replace what the loop wrote there.
+        if (!kForward && !none) te = weigh_entries(c, n, e, sh);
         __syncthreads();
         if (!none) {
             const float mass = static_cast<float>(te.mass);
             for (uint32_t k = threadIdx.x; k < n; k += kThreads) {
-                float t_sum;
-                if (!here(e.id[k]) || !first_of_id(e, unordered, n, k, t_sum)) continue;
+                if (!here(e.id[k]) || !first_of_id(e, unordered, k)) continue;
                 const float p = __fmul_rn(exp_fast(__fsub_rn(e.v[k], row_max)), inv);
-                g[e.id[k]] = from_float<T>(__fmul_rn(by, __fsub_rn(__fmul_rn(p, mass), t_sum)));
+                const float t = unordered ? sum_of_id(e, n, k) : e.t[k];
+                g[e.id[k]] = from_float<T>(__fmul_rn(by, __fsub_rn(__fmul_rn(p, mass), t)));
+            }
+        }
+    }
+    if (kForward && listed) {
+        cluster.barrier_wait();  // every CTA's part of the loss is here
+        if (rank == 0 && warp == 0) {
+            double loss = warp_sum(lane < ctas ? sh.share[lane].cross : 0.0);
+            const double held_all = warp_sum(lane < ctas ? sh.share[lane].held : 0.0);
+            if (lane == 0) {
+                const float mr = sh.red_m[0], sr = sh.red_s[0];
+                const double lse = static_cast<double>(sh.row.x) + log(static_cast<double>(sh.red_s[1]));
+                loss += held_all * (c.tail ? lse : lse - log(te.sum));
+                if (te.r > 0.0) {
+                    loss += te.r * (log(te.r) + lse);
+                    loss -= te.r * (sr != 0.0f ? static_cast<double>(mr) + log(static_cast<double>(sr))
+                                               : static_cast<double>(kNegInf));
+                }
+                c.loss[row] = te.some ? static_cast<float>(loss) : 0.0f;
             }
         }
     }
 }
 
-// Largest segment of the resident kernel (with its phase): one CTA an SM.
-constexpr size_t kResidentMax = 200u << 10;
-
-template <typename T, bool kForward, bool kGrad, bool kResident>
-cudaError_t launch(const DistillCall &c, uint32_t ctas, size_t buffer, cudaStream_t stream) {
-    buffer = (buffer + 15u) & ~size_t{15};
+template <typename T, bool kForward, bool kGrad>
+cudaError_t launch(const DistillCall &c, uint32_t ctas, size_t bitmap, cudaStream_t stream) {
+    bitmap = (bitmap + 15u) & ~size_t{15};
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(c.rows * ctas, 1, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
-    cfg.dynamicSmemBytes = buffer + c.cap * kEntryBytes;
+    cfg.dynamicSmemBytes = bitmap + c.cap * kEntryBytes;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -763,45 +699,41 @@ cudaError_t launch(const DistillCall &c, uint32_t ctas, size_t buffer, cudaStrea
     attr[0].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, distill_kernel<T, kForward, kGrad, kResident>, c, ctas,
-                              static_cast<uint32_t>(buffer));
+    return cudaLaunchKernelEx(&cfg, distill_kernel<T, kForward, kGrad>, c, ctas,
+                              static_cast<uint32_t>(bitmap));
 }
 
 template <typename T>
 cudaError_t launch_typed(const DistillCall &c, bool forward, bool grad, int num_sms,
                          cudaStream_t stream) {
-    // Four CTAs per SM, in segments of at least 2048 logits.
-    uint32_t ctas = 1;
-    while (ctas < kMaxCtas && static_cast<size_t>(c.rows) * ctas < 4u * static_cast<size_t>(num_sms) &&
+    const size_t bytes = static_cast<size_t>(c.vocab) * sizeof(T);
+    // A CTA's segment. The loss alone and the backward pass read a row once, and
+    // every CTA of a row repeats the work on its list: whole rows up to 320 KB
+    // (2 x 160 KB costs 4096 x 128256 bf16 losses 231 us against 199). Loss and
+    // gradient together read the row twice, the second time from L2, which has to
+    // hold what the CTAs of the GPU (six per SM) are at: 104 KB each (2048 x
+    // 151936 bf16: 259 us; 309 us with whole rows, which are read from HBM twice;
+    // 272 us with 52 KB). Small batches take more CTAs, to four per SM.
+    const size_t share = (forward && grad ? 104u : 320u) << 10;
+    uint32_t ctas = static_cast<uint32_t>(std::min<size_t>(kMaxCtas, (bytes + share - 1) / share));
+    while (ctas < kMaxCtas && static_cast<size_t>(c.rows) * ctas < 4 * static_cast<size_t>(num_sms) &&
            c.vocab / (ctas * 2) >= 2048)
-        ctas *= 2;
-    if (!forward) return launch<T, false, true, false>(c, ctas, 0, stream);
-    const auto seg_of = [&](uint32_t n) { return ((c.vocab + n - 1) / n + 31u) & ~31u; };
-    // Segments of at most 52 KB: four CTAs of an SM, some copying while others
-    // compute and write.
-    const size_t bytes = static_cast<size_t>(c.vocab) * sizeof(T), share = 52u << 10;
-    const uint32_t want = static_cast<uint32_t>(std::min<size_t>(kMaxCtas, (bytes + share - 1) / share));
-    const uint32_t resident = std::max(ctas, want);
-    const size_t smem = seg_of(resident) * sizeof(T) + 16;
-    if (grad && smem <= kResidentMax) return launch<T, true, true, true>(c, resident, smem, stream);
-    // The loss alone is streamed; wider rows are too, twice for their gradient.
-    // The bitmap of a segment fits in shared memory.
-    while (ctas < kMaxCtas && c.vocab / ctas > (1u << 20)) ctas *= 2;
-    const size_t bits = c.tail ? (seg_of(ctas) / 32u + 2u) * sizeof(uint32_t) : 0;
-    return grad ? launch<T, true, true, false>(c, ctas, bits, stream)
-                : launch<T, true, false, false>(c, ctas, bits, stream);
+        ctas = std::min(kMaxCtas, ctas * 2);
+    if (!forward) return launch<T, false, true>(c, ctas, 0, stream);
+    const uint32_t seg = ((c.vocab + ctas - 1) / ctas + 31u) & ~31u;
+    const size_t bits = c.tail ? (seg / 32u + 2u) * sizeof(uint32_t) : 0;
+    return grad ? launch<T, true, true>(c, ctas, bits, stream) : launch<T, true, false>(c, ctas, bits, stream);
 }
 
 template <typename T>
 cudaError_t setup_typed() {
-    const int most = static_cast<int>(kResidentMax + kDistillMaxTop * kEntryBytes);
-    cudaError_t e = cudaFuncSetAttribute(distill_kernel<T, true, true, true>,
+    // A bitmap of kDistillMaxVocab / kMaxCtas elements and the longest lists.
+    const int most = static_cast<int>((kDistillMaxVocab / kMaxCtas / 32u + 3u) * sizeof(uint32_t) +
+                                      kDistillMaxTop * kEntryBytes + 16u);
+    cudaError_t e = cudaFuncSetAttribute(distill_kernel<T, true, true>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(distill_kernel<T, true, true, false>,
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(distill_kernel<T, true, false, false>,
+        e = cudaFuncSetAttribute(distill_kernel<T, true, false>,
                                  cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     return e;
 }

@@ -109,6 +109,12 @@ def test_large_rows(dtype):
     check(*case(2, 151936, 64, seed=3, dtype=dtype), tail=True, temperature=2.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_wide_vocabularies(dtype):
+    """Segments far above 104 and 320 KB, at the largest cluster."""
+    check(*case(2, 1500003, 1024, seed=5, dtype=dtype), tail=True)
+
+
 @pytest.mark.parametrize("tail", [False, True])
 @pytest.mark.parametrize("rows", [149, 700])
 def test_many_rows(rows, tail):
