@@ -201,17 +201,29 @@ verify_greedy_rows_kernel(const __grid_constant__ VerifyCall c) {
     uint32_t lo, hi;
     part_bounds(c, r.part, lo, hi);
     unsigned long long best = 0;
-    uint32_t finite = 0;
+    uint32_t best_key = 0, finite = 0;
     auto visit = [&](uint32_t j, float x) {
-        const float v = masked_scaled(x, c.scale);
-        const unsigned long long cand = pack_key_index(total_key(v), j);
-        best = cand > best ? cand : best;
+        const uint32_t key = total_key(masked_scaled(x, c.scale));
+        if (key >= best_key) best_key = key, best = pack_key_index(key, j);
         finite |= fabsf(x) < kPosInf ? 1u : 0u;
     };
     const float *p = target_row(c, r.b, r.i);
     visit_segment<kRowThreads, 4>(
         p, lo, hi,
         [&](uint32_t body, uint32_t q0, const float4 *x) {
+            // The batch's largest key first: few batches hold a new maximum. A
+            // thread whose maximum is +inf looks on for finite logits; any other
+            // maximum above -inf is one.
+            uint32_t top = 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t a = max(total_key(masked_scaled(x[k].x, c.scale)),
+                                       total_key(masked_scaled(x[k].y, c.scale)));
+                const uint32_t b = max(total_key(masked_scaled(x[k].z, c.scale)),
+                                       total_key(masked_scaled(x[k].w, c.scale)));
+                top = max(top, max(a, b));
+            }
+            if (top < best_key && best_key < kKeyPosInf) return;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
                 const uint32_t j = body + 4u * (q0 + k * kRowThreads);

@@ -134,6 +134,7 @@ class Engine:
         if dev.index is None:
             dev = torch.device("cuda", torch.cuda.current_device())
         self.device = dev
+        self._index = dev.index  # what Tensor.get_device() gives there
         self.lib = _lib.lib()
         self._h = ctypes.c_void_p()
         self.max_rows = 0
@@ -398,7 +399,7 @@ class Engine:
     # -- verification of drafted tokens ---------------------------------------
     def _want(self, t: torch.Tensor, what: str, dtype: torch.dtype, shape) -> int:
         """The address of a dense argument of this type and shape on the engine's device."""
-        if t.dtype is dtype and t.shape == shape and t.device == self.device and t.is_contiguous():
+        if t.dtype is dtype and t.shape == shape and t.get_device() == self._index and t.is_contiguous():
             return t.data_ptr()
         if t.device != self.device:
             raise ValueError(f"{what} on {t.device}, engine on {self.device}")
@@ -411,9 +412,9 @@ class Engine:
     def _rows_3d(self, t: torch.Tensor, what: str, shape: tuple) -> tuple[int, int, int]:
         """(address, sequence stride, row stride) of [sequences, rows, vocab] f32 logits whose rows
         are contiguous; the strides may be larger than dense ones, and in either order."""
-        if t.device != self.device:
+        if t.get_device() != self._index:
             raise ValueError(f"{what} on {t.device}, engine on {self.device}")
-        if t.dtype != torch.float32:
+        if t.dtype is not torch.float32:
             raise TensorError("F32", str(t.dtype).replace("torch.", "").upper())
         if t.shape != shape:
             raise InvalidShape(list(t.shape))
@@ -554,22 +555,21 @@ class Engine:
                        n: Optional[torch.Tensor], temperature: float, tail: bool):
         """The C batch of [..., vocab] logits and [..., top] teacher entries, with the tensors it
         points into (kept until the call has been issued)."""
-        if logits.device != self.device:
+        if logits.get_device() != self._index:
             raise ValueError(f"logits on {logits.device}, engine on {self.device}")
         dtype = _DISTILL_TYPES.get(logits.dtype)
         if dtype is None:
             raise TensorError("f32, bf16 or f16", str(logits.dtype).replace("torch.", ""))
-        if logits.dim() < 1 or ids.shape[:-1] != logits.shape[:-1] or ids.dim() != logits.dim():
-            raise InvalidShape(list(ids.shape))
-        shape = logits.shape
-        lead, vocab, cap = shape[:-1], shape[-1], ids.shape[-1]
-        rows = lead.numel()
+        shape, entries = logits.shape, ids.shape
+        lead = shape[:-1]
+        if len(shape) < 1 or len(entries) != len(shape) or entries[:-1] != lead:
+            raise InvalidShape(list(entries))
+        vocab, cap, rows = shape[-1], entries[-1], lead.numel()
         x = logits if len(shape) == 2 else logits.reshape(rows, vocab)
         stride, step = x.stride()
         if rows > 0 and vocab > 1 and (step != 1 or (rows > 1 and stride < vocab)):
             x = x.contiguous()  # rows out of order, or one row broadcast to many
             stride = vocab
-        entries = (*lead, cap)
         return _lib.RscDistillBatch(
             rows, vocab, x.data_ptr(), stride if rows > 1 else vocab, dtype, bool(tail), temperature,
             cap, None if n is None else self._want(n, "n", torch.int32, lead),
@@ -601,7 +601,7 @@ class Engine:
         b, x = self._distill_batch(logits, ids, logprobs, n, temperature, tail)
         up = self._want(row_grads, "row_grads", torch.float32, logits.shape[:-1])
         if out is None:
-            out = torch.empty(logits.shape, dtype=logits.dtype, device=self.device)
+            out = torch.empty_like(logits, memory_format=torch.contiguous_format)
             stride = b.vocab
         else:
             if out is not logits:
@@ -624,7 +624,7 @@ class Engine:
         b, x = self._distill_batch(logits, ids, logprobs, n, temperature, tail)
         up = self._want(row_grads, "row_grads", torch.float32, logits.shape[:-1])
         st = self._want(state, "state", torch.float32, (b.rows, 4))
-        grad = torch.empty(logits.shape, dtype=logits.dtype, device=self.device)
+        grad = torch.empty_like(logits, memory_format=torch.contiguous_format)
         check(self.lib.rsc_distill_backward(self._h, ctypes.byref(b), st, up, grad.data_ptr(), b.vocab,
                                             _stream_ptr(self.device)), "rsc_distill_backward")
         return grad
@@ -692,6 +692,9 @@ _ENGINES: dict[int, Engine] = {}
 
 def engine(device: int | torch.device | None = None) -> Engine:
     """The shared Engine of a device."""
+    e = _ENGINES.get(device) if type(device) is int else None
+    if e is not None:
+        return e
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     idx = dev.index if dev.index is not None else torch.cuda.current_device()
     if idx not in _ENGINES:

@@ -257,6 +257,32 @@ def test_output_distribution():
     assert (np.abs(share - p) < 6 * np.sqrt(p * (1 - p) / n)).all()
 
 
+@pytest.mark.parametrize("draft", [True, False])
+def test_large_batches(draft):
+    """Several waves of row parts; what lies behind a sequence's first refused position does not
+    matter, NaN neither."""
+    b, d, v = 24, 8, 50003
+    x, y, t, u = case(b, d, v, seed=111, draft=draft)
+    n = np.random.default_rng(112).integers(0, d + 1, size=b).astype(np.int32)
+    t[3, 2] = v                                   # outside the vocabulary
+    x[5, 1] = -np.inf
+    t[7] = x[7, :d].argmax(1)
+    u[7, :d] = 0.0                                # accepts to the end
+    n[7] = d
+    for i in range(12, b):
+        u[i, :i % (d + 1)] = 0.0                  # accepts at least these
+    want = R.verify_batch(x, y, t, n, u, 1.0)
+    assert len(set(want[1])) > 3
+    same(run(x, y, t, u, n=n), want)
+    for i in range(b):
+        x[i, want[1][i] + 1:] = np.nan
+    same(run(x, y, t, u, n=n), want)
+    t = np.where(np.random.default_rng(113).random(t.shape) < 0.7, np.nan_to_num(x[:, :d]).argmax(2), t).astype(np.int32)
+    greedy = R.greedy_batch(x, t, n)
+    out = engine(0).verify(dev(x), dev(t), SamplingParams(0.0), n_draft=dev(n))
+    same([o.cpu().numpy() for o in out], greedy)
+
+
 def test_streams_graphs_and_reused_outputs():
     b, d, v = 6, 3, 30011
     sets = [case(b, d, v, seed=81 + k) for k in range(2)]

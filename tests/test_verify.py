@@ -43,6 +43,7 @@ def cpu_engine() -> Engine:
     e = Engine.__new__(Engine)
     e.device, e.lib, e._h = torch.device("cpu"), _lib.lib(), ctypes.c_void_p()
     e.max_rows = e.max_vocab = 0
+    e._index = -1  # Tensor.get_device() on the CPU
     return e
 
 
