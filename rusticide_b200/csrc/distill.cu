@@ -348,9 +348,9 @@ __device__ __forceinline__ float batch_sum(const uint4 *w, uint64_t c, uint64_t 
     return __fadd_rn(low_of(e[0]), high_of(e[0]));
 }
 
-// (m, s) of this thread's share of a segment in global memory: a batch of
-// 16-byte words at a time against one running maximum. Where the tail is wanted
-// by itself the listed elements are left out by their bit.
+// (m, s) of this thread's share of a segment: a batch of 16-byte words at a time
+// against one reference, as in rsc_rowsum.cuh. Where the tail is wanted by itself
+// the listed elements are left out by their bit.
 template <typename T>
 __device__ __forceinline__ void sum_segment(const DistillCall &c, const T *x, const Segment<T> &seg,
                                              uint32_t *bits, const Entries &en, uint32_t n, float &m,
@@ -380,8 +380,10 @@ __device__ __forceinline__ void sum_segment(const DistillCall &c, const T *x, co
     if (threadIdx.x >= 32 && threadIdx.x - 32 < hi - seg.tail) j = seg.tail + threadIdx.x - 32;
     if (j < hi && !(masked && (bits[(j - lo + pad) / 32u] >> ((j - lo + pad) % 32u) & 1u)))
         one = elem_to_float<T>(x[j]);
-    float top = one;
-    ExpRef r(c, top > kNegInf ? __fmul_rn(top, c.scale) : 0.0f);
+    // m stays -inf until there is a logit above it; the exponents' reference is
+    // then 0, against which -inf gives 0 and NaN gives NaN.
+    if (one > kNegInf) m = __fmul_rn(one, c.scale);
+    ExpRef r(c, m > kNegInf ? m : 0.0f);
     double correction = r.correction(c);
     s = static_cast<double>(exp_one(one, c.scale, r)) * correction;
     const uint4 *words = reinterpret_cast<const uint4 *>(x + seg.body);
@@ -408,11 +410,11 @@ __device__ __forceinline__ void sum_segment(const DistillCall &c, const T *x, co
         float b = word_max<T>(w[0]);
 #pragma unroll
         for (int k = 1; k < kN; ++k) b = fmaxf(b, word_max<T>(w[k]));
-        if (b > top) {
-            const float next = __fmul_rn(b, c.scale);
+        const float next = __fmul_rn(b, c.scale);
+        if (next > m + kHeadroom) {
             // Before the first logit above -inf the sum is 0 or NaN.
-            if (top > kNegInf) s *= static_cast<double>(exp_fast(__fsub_rn(r.ref, next)));
-            top = b;
+            if (m > kNegInf) s *= static_cast<double>(exp_fast(__fsub_rn(m, next)));
+            m = next;
             r = ExpRef(c, next);
             correction = r.correction(c);
         }
@@ -445,7 +447,6 @@ __device__ __forceinline__ void sum_segment(const DistillCall &c, const T *x, co
         const uint32_t set = listed(q0);
         add(&w, &set, std::integral_constant<int, 1>());
     }
-    m = top > kNegInf ? r.ref : kNegInf;
 }
 
 template <typename T, bool kForward, bool kGrad>

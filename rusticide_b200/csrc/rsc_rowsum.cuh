@@ -1,14 +1,16 @@
 // Running log-sum-exp of a row segment, shared by the kernels that read whole
 // rows of logits (draft verification, distillation).
 //
-// A partial sum is the pair (m, s): m the largest scaled logit seen, s the sum
-// of exp(v - m) over the segment. A thread takes its logits in batches of 16:
-// the batch's maximum first, then sixteen exponentials against one running
-// maximum, added as a tree in binary32 and once per batch into a binary64 sum.
-// The tree is four additions deep, so a sum is off by at most 4 half-ulps plus
-// the exponentials' own error: exp(v - m) is ex2.approx of a product rounded
-// once, |v - m| * 2^-23 + 2^-22 relative. With |v - m| below 25 for every term
-// that counts, that is under 4e-6 in all.
+// A partial sum is the pair (m, s): s the sum of exp(v - m) over the segment, m
+// a reference at most kHeadroom below the largest v. A thread takes its logits in
+// batches of 16: the batch's maximum first, then sixteen exponentials against one
+// reference, added as a tree in binary32 and once per batch into a binary64 sum.
+// Its error has three parts. An exponential is ex2.approx of a product rounded
+// once, |v - m| 2^-23 + 2^-22 relative. A new reference, and the join of lanes,
+// warps and parts, scales a sum by one more of them; references rise by more than
+// kHeadroom, so the terms that count, within 25 of the largest, see at most six,
+// and their distances add up to that 25: 3e-6 + 10 * 2^-22 in all. The trees are
+// four additions deep (2^-22). Together below 6e-6.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -64,12 +66,14 @@ __device__ __forceinline__ void unpack<__half>(const uint4 &w, float *f) {
     }
 }
 
-// exp(d) for d <= 0: ex2.approx of the product with log2(e).
+// exp(d): ex2.approx of the product with log2(e).
 __device__ __forceinline__ float exp_fast(float d) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fmul_rn(d, 1.4426950408889634f)));
     return r;
 }
+
+constexpr float kHeadroom = 4.0f;
 
 // Adds kN scaled logits to (m, s). A logit of -inf adds nothing; +inf makes m
 // +inf and s NaN, and NaN makes s NaN (callers that read NaN as -inf fold it
@@ -79,7 +83,7 @@ __device__ __forceinline__ void sum_batch(float &m, double &s, const float *v) {
     float b = v[0];
 #pragma unroll
     for (int i = 1; i < kN; ++i) b = fmaxf(b, v[i]);
-    if (b > m) {
+    if (b > m + kHeadroom) {
         // m = -inf only while s is 0 or NaN, which the product keeps.
         s *= m == kNegInf ? 1.0 : static_cast<double>(exp_fast(__fsub_rn(m, b)));
         m = b;
@@ -98,21 +102,8 @@ __device__ __forceinline__ void sum_batch(float &m, double &s, const float *v) {
     s = __dadd_rn(s, static_cast<double>(e[0]));
 }
 
-// (m, s) joined with (m2, s2).
-__device__ __forceinline__ void sum_join(float &m, double &s, float m2, double s2) {
-    if (m2 > m) {
-        s = (m == kNegInf ? s : s * exp(static_cast<double>(m) - static_cast<double>(m2))) + s2;
-        m = m2;
-    } else if (m2 == kNegInf || m2 == m) {
-        s += s2;  // 0 or NaN against -inf; equal maxima need no factor
-    } else {
-        s += s2 * exp(static_cast<double>(m2) - static_cast<double>(m));
-    }
-}
-
 // The sums of `width` neighbouring lanes joined, in every one of them: the
-// maximum first, then each lane's sum brought to it by one exponential (whose
-// error, as a batch's, is within 4e-6).
+// largest reference first, then each lane's sum brought to it by one exponential.
 __device__ __forceinline__ void sum_join_lanes(float &m, double &s, int width) {
     float top = m;
     for (int o = width / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));

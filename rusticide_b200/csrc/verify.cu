@@ -18,8 +18,9 @@
 //
 // Whole vocabulary, two launches:
 //  1. verify_rows_kernel reads the rows of every test once (HBM-bound) and
-//     leaves a binary32 (maximum, sum) per row part; position-major, so that
-//     large batches can skip the rows behind a refused token.
+//     leaves a binary32 (reference, sum) per row part. (Ending a sequence's
+//     rows at a refusal seen meanwhile was tried: its flags and counters cost
+//     what it saved, 126 us against 123 at 96 x 7 x 128256.)
 //  2. verify_draw_kernel, one cluster per sequence: decides the tests from
 //     those sums where their error bound allows it, sums the first undecided
 //     or refused position's rows once more in binary64, decides it exactly, and
@@ -43,9 +44,9 @@ constexpr int kDrawThreads = 256;
 constexpr int kDrawWarps = kDrawThreads / 32;
 constexpr uint32_t kDrawMaxCtas = 16;  // the largest cluster (8 is the largest portable one)
 
-// Part of a row, as the first launch leaves it: (maximum, sum of exp(v -
-// maximum)), or for greedy calls the packed (total-order key, index) of the
-// largest logit and whether any logit is finite.
+// Part of a row, as the first launch leaves it: (m, sum of exp(v - m)) with m
+// near the largest v (rsc_rowsum.cuh), or for greedy calls the packed
+// (total-order key, index) of the largest logit and whether any logit is finite.
 struct RowPart {
     union {
         float max;
@@ -111,14 +112,17 @@ __device__ __forceinline__ void visit_segment(const float *p, uint32_t lo, uint3
 }
 
 // ---------------------------------------------------------------------------
-// Launch 1: a CTA per row part.
+// Launch 1: a CTA per row part. Bound by HBM, with sixteen exponentials' worth
+// of loads in flight a thread: 96 x 7 x 128256 with ragged drafts reads 345 MB in
+// some 57 us (6 TB/s); the greedy form of 64 x 4 x 151936, 195 MB, in 38 us (5.1
+// TB/s, the same with 2, 4 and 8 loads in flight and with 4 to 16 parts a row).
 // ---------------------------------------------------------------------------
 struct RowItem {
     uint32_t b, i, part;
     bool draft;
 };
 
-// Block index -> (position, sequence, row kind, part), positions slowest.
+// Block index -> (position, sequence, row kind, part).
 __device__ __forceinline__ RowItem row_item(const VerifyCall &c, uint32_t kinds) {
     uint32_t x = blockIdx.x;
     RowItem r;
@@ -254,7 +258,8 @@ verify_greedy_rows_kernel(const __grid_constant__ VerifyCall c) {
 }
 
 // ---------------------------------------------------------------------------
-// Greedy verification, launch 2: one warp per sequence.
+// Greedy verification, launch 2: one warp per sequence. It reads a few words a
+// row and is bound by their latency.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(128)
 verify_greedy_kernel(const __grid_constant__ VerifyCall c) {
@@ -293,38 +298,44 @@ verify_greedy_kernel(const __grid_constant__ VerifyCall c) {
 // Launch 2: decisions and the last token.
 // ---------------------------------------------------------------------------
 
-// What exp(v - max) of a row is taken with. Terms that far below the maximum
-// (-inf and NaN among them) that exp would leave binary64 are held at exp(-700),
-// 1e-304, so that no term needs a branch: no sum that counts feels it. Weights
-// up to kNoWeight are those of such terms.
+// What exp(v - max) of a row is taken with; `max` is a reference that v exceeds
+// by 600 at most. Scaled logits more than 700 below it (-inf and NaN among them)
+// are raised to that floor, so that no term needs a branch; weights up to
+// kNoWeight, of terms 460 or more below it, count as 0 where a draw asks for the
+// first of any weight. Beyond 2^33
+// neighbouring binary32 numbers are 1024 apart: such a row is scaled down to
+// where they are 512 apart and the floor is next to the maximum, which leaves
+// every other token without weight, as it is.
 struct RowBase {
-    float scale, max32;
+    float scale, max32, floor;
     double max;
     __device__ __forceinline__ RowBase() {}
-    __device__ __forceinline__ RowBase(float scale_, float max_) : scale(scale_), max32(max_), max(max_) {}
+    __device__ __forceinline__ RowBase(float scale_, float max_) : scale(scale_), max32(max_) {
+        if (fabsf(max_) >= 0x1p+33f) {
+            const float down = scalbnf(1.0f, 32 - ilogbf(max_));
+            scale *= down;
+            max32 *= down;
+        }
+        floor = max32 - 700.0f;
+        max = max32;
+    }
 };
-constexpr double kNoWeight = 1e-280;
+constexpr double kNoWeight = 1e-200;
 
 constexpr uint32_t kExpSteps = 512;  // entries of the table 2^(j / kExpSteps)
 
 // exp(v - max) in binary64, v = x * scale. With d = v - max = k ln2 / 512 + r
 // it is 2^(k/512) * (1 + r + r^2/2 + r^3/6); k comes from d in binary32, which
 // leaves |r| below 0.6 ln2 / 512 = 8.2e-4, and the first neglected term, r^4/24,
-// below 2e-14. What bounds a pass is the chain of dependent binary64 operations
-// (and their rate, 16 lanes a cycle and scheduler), so k does not wait for
-// them and the polynomial is two deep. d <= 0 apart from a row summed against
-// its first block; negative ones order by magnitude in their high words, so
-// the nearer of d and -700 is an integer minimum (positive ones pass it).
+// below 2e-14. What bounds a pass is the count of instructions (25 with the
+// load), then the binary64 rate (six operations at 16 lanes a cycle and
+// scheduler), so k is found beside them and the polynomial is two deep.
 __device__ __forceinline__ double exp64(float x, const RowBase &b, const double *tab) {
-    const float v = masked_scaled(x, b.scale);
-    const double far = __dsub_rn(static_cast<double>(v), b.max);
-    const uint32_t high = min(static_cast<uint32_t>(__double2hiint(far)), 0xc085e000u);  // -700
-    const double d = __hiloint2double(static_cast<int>(high), __double2loint(far));
-    const float kf = __fmaf_rn(fmaxf(__fsub_rn(v, b.max32), -700.0f), kExpSteps * 1.44269504f, 0x1.8p+23f);
+    const float v = fmaxf(__fmul_rn(x, b.scale), b.floor);  // NaN gives the floor
+    const float kf = __fmaf_rn(__fsub_rn(v, b.max32), kExpSteps * 1.44269504f, 0x1.8p+23f);
     const uint32_t k = __float_as_uint(kf) - 0x4b400000u;
-    // 2^52 + 2^31 + k, less 2^52 + 2^31.
-    const double kd = __dsub_rn(__hiloint2double(0x43300000, static_cast<int>(k ^ 0x80000000u)),
-                                0x1p+52 + 0x1p+31);
+    const double kd = static_cast<double>(__fsub_rn(kf, 0x1.8p+23f));
+    const double d = __dsub_rn(static_cast<double>(v), b.max);
     const double r = __fma_rn(kd, -0.69314718055994530942 / kExpSteps, d);
     const double p = __fma_rn(__dmul_rn(r, r), __fma_rn(r, 1.0 / 6.0, 0.5), r);
     const double t = tab[k % kExpSteps];
@@ -891,7 +902,11 @@ verify_draw_kernel(const __grid_constant__ VerifyCall c, uint32_t ctas) {
 }
 
 // ---------------------------------------------------------------------------
-// Survivor records: one block per sequence.
+// Survivor records: one block per sequence, a warp per test, then one warp that
+// draws. The lists are short (top_k and its ties), so the call is bound by the
+// chain of dependent loads (token, list, bisection in the draft's list) and the
+// launch: one sequence of 4 drafts over 64 slots 5.5 us, 512 of 6 over 152 slots
+// 14.6 us.
 // ---------------------------------------------------------------------------
 constexpr int kListThreads = 128;
 constexpr int kListWarps = kListThreads / 32;
@@ -1059,7 +1074,7 @@ size_t verify_workspace_bytes(size_t n_seqs, size_t max_drafts, size_t vocab) {
 // of it finds room); more take slices of about 24576 tokens, whose uneven
 // lengths (a refused token reads two rows, an accepted draft one) even out.
 // Measured, us a call: 8 x 5 x 151936 27.5 with 16 CTAs, 35.7 with 8; 32 x 8 x
-// 50001 20.5 with 6, 25.8 with 8; 96 x 7 x 128256 123 with 6, 138 with 2.
+// 50001 20.3 with 6, 25.8 with 8; 96 x 7 x 128256 120 with 6, 138 with 2.
 uint32_t draw_ctas(uint32_t n_seqs, uint32_t vocab, int num_sms) {
     const uint32_t room = static_cast<uint32_t>(num_sms) * 4u / 3u / n_seqs;
     uint32_t ctas = room >= 16 ? 16u : std::min(room, 8u);

@@ -13,13 +13,19 @@ from typing import Optional
 
 import torch
 
-from .sampler import engine
+from .sampler import Engine, engine
+
+
+def _engine_of(logits: torch.Tensor) -> Engine:
+    if not logits.is_cuda:
+        raise RuntimeError("distill_loss needs logits on a CUDA device; there is no CPU fallback")
+    return engine(logits.get_device())
 
 
 class _DistillLoss(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, logprobs, n, temperature, tail):
-        loss, state = engine(logits.get_device()).distill_forward(logits, ids, logprobs, n, temperature, tail)
+        loss, state = _engine_of(logits).distill_forward(logits, ids, logprobs, n, temperature, tail)
         ctx.save_for_backward(logits, ids, logprobs, n, state)
         ctx.how = (temperature, tail)
         return loss
@@ -28,7 +34,7 @@ class _DistillLoss(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad_loss):
         logits, ids, logprobs, n, state = ctx.saved_tensors
-        grad = engine(logits.get_device()).distill_backward(
+        grad = _engine_of(logits).distill_backward(
             logits, ids, logprobs, state, grad_loss.contiguous(), n, *ctx.how)
         return grad, None, None, None, None, None
 
@@ -43,5 +49,5 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor
     `Engine.distill_step`, which gives loss and gradient in one pass."""
     if logits.requires_grad and torch.is_grad_enabled():
         return _DistillLoss.apply(logits, ids, logprobs, n, temperature, tail)
-    return engine(logits.get_device()).distill_forward(logits, ids, logprobs, n, temperature, tail,
+    return _engine_of(logits).distill_forward(logits, ids, logprobs, n, temperature, tail,
                                                  want_state=False)[0]

@@ -600,6 +600,7 @@ class Engine:
         itself, which the gradient then replaces."""
         b, x = self._distill_batch(logits, ids, logprobs, n, temperature, tail)
         up = self._want(row_grads, "row_grads", torch.float32, logits.shape[:-1])
+        written = out is not None
         if out is None:
             out = torch.empty_like(logits, memory_format=torch.contiguous_format)
             stride = b.vocab
@@ -614,6 +615,8 @@ class Engine:
         loss = logprobs.new_empty(logits.shape[:-1])
         check(self.lib.rsc_distill(self._h, ctypes.byref(b), loss.data_ptr(), None, up, out.data_ptr(),
                                    stride, _stream_ptr(self.device)), "rsc_distill")
+        if written:
+            torch.autograd.graph.increment_version(out)  # a graph that saved it must not go on
         return loss, out
 
     def distill_backward(self, logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor,

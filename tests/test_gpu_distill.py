@@ -1,11 +1,11 @@
 """Distillation on the GPU against the binary64 form of distill_ref.py.
 
-Tolerances, from the arithmetic (rsc_rowsum.cuh): a sum of exponentials is within 4e-6 relative, so a
-log of it within 4e-6, and the loss, which holds at most two of them with weights that add up to
+Tolerances, from the arithmetic (rsc_rowsum.cuh): a sum of exponentials is within 6e-6 relative, so a
+log of it within 6e-6, and the loss, which holds at most two of them with weights that add up to
 1 + r <= 2, within 1.2e-5, plus a binary32 rounding of t (2^-24 relative of terms that add up to less
-than 40 here) and of the result. A gradient's p has |v - m| 2^-23 + 2^-22 from its exponential
-(|v - m| < 60 here: 8e-6), 4e-6 from the sum and four roundings: 1.3e-5 relative, and so has the
-tail's r exp(v) / S_tail. The result is rounded to its type by at most half a step, relative eps / 2
+than 40 here) and of the result. A gradient's p has |v - m| 2^-22 + 2^-22 from its exponential
+(|v - m| < 25 here where p is a normal number of the result: 6.2e-6), 6e-6 from the sum and four
+roundings (2.4e-7): 1.3e-5 relative, and so has the tail's r exp(v) / S_tail. The result is rounded to its type by at most half a step, relative eps / 2
 or half the smallest subnormal."""
 
 import numpy as np
