@@ -22,8 +22,8 @@
 // summed over the unlisted tokens as such (a bitmap of the listed ones masks
 // them out): S minus the listed terms would lose it where the listed tokens
 // hold nearly all of the mass. Measured (B200, GPU time): loss of 4096 x 128256
-// bf16 with 128 entries and the tail 199 us (5.3 TB/s), loss and gradient of 2048
-// x 151936 bf16 259 us (4.8 TB/s of one read and one write). Keeping the segment
+// bf16 with 128 entries and the tail 187 us (5.6 TB/s), loss and gradient of 2048
+// x 151936 bf16 231 us (5.4 TB/s of one read and one write). Keeping the segment
 // in shared memory between the passes (TMA copies, four CTAs of 52 KB an SM)
 // took 305-322 us: the phases of so few CTAs do not overlap.
 #include <algorithm>
@@ -313,6 +313,54 @@ __device__ __forceinline__ void join_lanes(float &m, float &s) {
     m = top;
 }
 
+// Loss and gradient together: a thread's own words of a segment on their way
+// through shared memory, kDepth batches of kBatch 16-byte words copied
+// asynchronously, so that the next ones travel while one is worked on. No other
+// thread reads them. The second pass goes from the segment's end, whose last
+// batches are still there. 48 KB a CTA leave four on an SM: 2048 x 151936 bf16
+// 233 us, against 258 with plain loads and six CTAs, 245 with six of 32 KB, 254 with
+// three of 64 KB, 240 with twelve words in batches of two. (The loss alone has no
+// second pass that stalls: six CTAs of plain loads, 188 us against 196 at 4096 x
+// 128256 bf16.)
+constexpr uint32_t kBatch = 4;
+constexpr uint32_t kDepth = 3;
+constexpr uint32_t kRingBytes = kThreads * kBatch * kDepth * 16;
+struct Ring {
+    const uint4 *from;  // this thread's first word
+    uint32_t slots;     // shared-memory address of its first slot
+    uint32_t full;      // whole batches of this thread
+
+    __device__ __forceinline__ Ring(const uint4 *words, uint32_t n_vec, unsigned char *smem)
+        : from(words + threadIdx.x),
+          slots(static_cast<uint32_t>(__cvta_generic_to_shared(smem)) + threadIdx.x * 16u) {
+        const uint32_t last = threadIdx.x + kThreads * (kBatch - 1);
+        full = n_vec > last ? (n_vec - last + kThreads * kBatch - 1) / (kThreads * kBatch) : 0u;
+    }
+    __device__ __forceinline__ uint32_t slot(uint32_t b) const {
+        return slots + (b % kDepth) * (kThreads * kBatch * 16u);
+    }
+    __device__ __forceinline__ void fetch(uint32_t b) const {
+        const uint4 *src = from + static_cast<size_t>(b) * (kThreads * kBatch);
+#pragma unroll
+        for (uint32_t k = 0; k < kBatch; ++k)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(slot(b) + k * kThreads * 16u),
+                         "l"(src + k * kThreads)
+                         : "memory");
+    }
+    static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+    static __device__ __forceinline__ void wait() {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kDepth - 1) : "memory");
+    }
+    __device__ __forceinline__ void take(uint32_t b, uint4 *w) const {
+#pragma unroll
+        for (uint32_t k = 0; k < kBatch; ++k)
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[k].x), "=r"(w[k].y), "=r"(w[k].z), "=r"(w[k].w)
+                         : "r"(slot(b) + k * kThreads * 16u)
+                         : "memory");
+    }
+};
+
 // A row segment of T cut at 16-byte boundaries: [lo, body) and [tail, hi)
 // element by element, n_vec 16-byte words from body on.
 template <typename T>
@@ -351,13 +399,20 @@ __device__ __forceinline__ float batch_sum(const uint4 *w, uint64_t c, uint64_t 
 // (m, s) of this thread's share of a segment: a batch of 16-byte words at a time
 // against one reference, as in rsc_rowsum.cuh. Where the tail is wanted by itself
 // the listed elements are left out by their bit.
-template <typename T>
+template <typename T, bool kRinged>
 __device__ __forceinline__ void sum_segment(const DistillCall &c, const T *x, const Segment<T> &seg,
-                                             uint32_t *bits, const Entries &en, uint32_t n, float &m,
-                                             double &s) {
+                                             uint32_t *bits, const Entries &en, uint32_t n, const Ring &ring,
+                                             float &m, double &s) {
     constexpr uint32_t kE = kVecElems<T>;
     const uint32_t lo = seg.lo, hi = seg.hi;
     const bool masked = c.tail;
+    if (kRinged) {
+#pragma unroll
+        for (uint32_t b = 0; b < kDepth; ++b) {
+            if (b < ring.full) ring.fetch(b);
+            Ring::commit();
+        }
+    }
     // Bit b stands for element lo - pad + b, so that the words' elements start at
     // bit 32 * first.
     const uint32_t first = (seg.body - lo + 31u) / 32u;
@@ -433,14 +488,28 @@ __device__ __forceinline__ void sum_segment(const DistillCall &c, const T *x, co
         return kE == 8 ? bytes[q] : bytes[q / 2u] >> (4u * (q & 1u)) & 15u;
     };
     uint32_t q0 = threadIdx.x;
-    for (; q0 + kThreads * (kLoads - 1) < seg.n_vec; q0 += kThreads * kLoads) {
-        uint4 w[kLoads];
-        uint32_t set[kLoads];
+    if (!kRinged) {
+        for (; q0 + kThreads * (kLoads - 1) < seg.n_vec; q0 += kThreads * kLoads) {
+            uint4 w[kLoads];
+            uint32_t set[kLoads];
 #pragma unroll
-        for (uint32_t k = 0; k < kLoads; ++k) w[k] = __ldg(words + q0 + k * kThreads);
+            for (uint32_t k = 0; k < kLoads; ++k) w[k] = __ldg(words + q0 + k * kThreads);
 #pragma unroll
-        for (uint32_t k = 0; k < kLoads; ++k) set[k] = listed(q0 + k * kThreads);
-        add(w, set, std::integral_constant<int, kLoads>());
+            for (uint32_t k = 0; k < kLoads; ++k) set[k] = listed(q0 + k * kThreads);
+            add(w, set, std::integral_constant<int, kLoads>());
+        }
+    }
+#pragma unroll 1
+    for (uint32_t b = 0; kRinged && b < ring.full; ++b, q0 += kThreads * kBatch) {
+        uint4 w[kBatch];
+        uint32_t set[kBatch];
+#pragma unroll
+        for (uint32_t k = 0; k < kBatch; ++k) set[k] = listed(q0 + k * kThreads);
+        Ring::wait();
+        ring.take(b, w);
+        if (b + kDepth < ring.full) ring.fetch(b + kDepth);
+        Ring::commit();
+        add(w, set, std::integral_constant<int, kBatch>());
     }
     for (; q0 < seg.n_vec; q0 += kThreads) {
         uint4 w = __ldg(words + q0);
@@ -450,7 +519,7 @@ __device__ __forceinline__ void sum_segment(const DistillCall &c, const T *x, co
 }
 
 template <typename T, bool kForward, bool kGrad>
-__global__ void __launch_bounds__(kThreads, kForward ? 6 : 8)
+__global__ void __launch_bounds__(kThreads, kForward ? (kGrad ? 4 : 6) : 8)
 distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bitmap_bytes) {
     // One bit per element of the segment (with the tail), then the entries.
     extern __shared__ __align__(16) unsigned char dynamic[];
@@ -463,8 +532,10 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bi
     const uint32_t seg_len = ((c.vocab + ctas - 1) / ctas + 31u) & ~31u;
     const uint32_t lo = min(c.vocab, rank * seg_len), hi = min(c.vocab, lo + seg_len);
     const Segment<T> seg(x, lo, hi);
+    constexpr uint32_t kRing = kForward && kGrad ? kRingBytes : 0;
+    const Ring ring(reinterpret_cast<const uint4 *>(x + seg.body), seg.n_vec, dynamic);
     Entries e;
-    e.id = reinterpret_cast<uint32_t *>(dynamic + bitmap_bytes);
+    e.id = reinterpret_cast<uint32_t *>(dynamic + kRing + bitmap_bytes);
     e.y = reinterpret_cast<float *>(e.id + c.cap);
     e.t = e.y + c.cap;
     e.v = e.t + c.cap;
@@ -473,8 +544,9 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bi
     // A row with an empty list is not looked at (for every CTA of the cluster alike).
     const bool listed = n > 0;
     float *state = c.state ? c.state + row * 4 : nullptr;
-    // Every CTA of the cluster runs before its memory is written.
-    if (kForward && listed) cluster.barrier_arrive();
+    // Every CTA of the cluster runs before its memory is written. (Warps that
+    // have written nothing for their peers arrive without a fence: 235 to 231 us.)
+    if (kForward && listed) asm volatile("barrier.cluster.arrive.relaxed.aligned;");
     if (threadIdx.x == 0) sh.unordered = 0;
     __syncthreads();
     load_entries(c, row, n, e, sh);
@@ -492,7 +564,7 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bi
     if (kForward && listed) {
         float m = kNegInf;
         double sum = 0.0;
-        sum_segment<T>(c, x, seg, reinterpret_cast<uint32_t *>(dynamic), e, n, m, sum);
+        sum_segment<T, kGrad>(c, x, seg, reinterpret_cast<uint32_t *>(dynamic + kRing), e, n, ring, m, sum);
         float s = static_cast<float>(sum);
         join_lanes(m, s);
         if (lane == 0) {
@@ -536,7 +608,10 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bi
             }
         }
         // The teacher's side while the cluster's other CTAs arrive.
-        cluster.barrier_arrive();
+        if (warp == 0)
+            cluster.barrier_arrive();
+        else
+            asm volatile("barrier.cluster.arrive.relaxed.aligned;");
         te = weigh_entries(c, n, e, sh);
         __syncthreads();
         cluster.barrier_wait();
@@ -558,7 +633,10 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bi
                 to.held = held_t;
             }
         }
-        cluster.barrier_arrive();
+        if (warp == 1)
+            cluster.barrier_arrive();
+        else
+            asm volatile("barrier.cluster.arrive.relaxed.aligned;");
         if (warp == 0 && (kGrad || rank == 0)) {
             const bool in = lane < ctas;
             float mr = in ? sh.share[lane].max_rest : kNegInf;
@@ -637,7 +715,22 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bi
                     out[q] = grad_word<T, true>(words[q], c.scale, r, factor);
             } else {
                 uint32_t q0 = threadIdx.x;
-                for (; q0 + kThreads * (kLoads - 1) < seg.n_vec; q0 += kThreads * kLoads) {
+                if (kForward) {
+                    // From the segment's end, whose last batches are still there.
+#pragma unroll 1
+                    for (uint32_t b = ring.full; b-- > 0;) {
+                        uint4 w[kBatch];
+                        Ring::wait();
+                        ring.take(b, w);
+                        if (b >= kDepth) ring.fetch(b - kDepth);
+                        Ring::commit();
+#pragma unroll
+                        for (uint32_t k = 0; k < kBatch; ++k)
+                            __stcs(out + q0 + (b * kBatch + k) * kThreads, grad_word<T, false>(w[k], c.scale, r, factor));
+                    }
+                    q0 += ring.full * kThreads * kBatch;
+                }
+                for (; !kForward && q0 + kThreads * (kLoads - 1) < seg.n_vec; q0 += kThreads * kLoads) {
                     uint4 w[kLoads];
 #pragma unroll
                     for (uint32_t k = 0; k < kLoads; ++k) w[k] = __ldcs(words + q0 + k * kThreads);
@@ -691,7 +784,7 @@ cudaError_t launch(const DistillCall &c, uint32_t ctas, size_t bitmap, cudaStrea
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(c.rows * ctas, 1, 1);
     cfg.blockDim = dim3(kThreads, 1, 1);
-    cfg.dynamicSmemBytes = bitmap + c.cap * kEntryBytes;
+    cfg.dynamicSmemBytes = (kForward && kGrad ? kRingBytes : 0) + bitmap + c.cap * kEntryBytes;
     cfg.stream = stream;
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -712,9 +805,8 @@ cudaError_t launch_typed(const DistillCall &c, bool forward, bool grad, int num_
     // every CTA of a row repeats the work on its list: whole rows up to 320 KB
     // (2 x 160 KB costs 4096 x 128256 bf16 losses 231 us against 199). Loss and
     // gradient together read the row twice, the second time from L2, which has to
-    // hold what the CTAs of the GPU (six per SM) are at: 104 KB each (2048 x
-    // 151936 bf16: 259 us; 309 us with whole rows, which are read from HBM twice;
-    // 272 us with 52 KB). Small batches take more CTAs, to four per SM.
+    // hold what the CTAs of the GPU (four per SM) are at: 104 KB each (2048 x
+    // 151936 bf16: 233 us; 243 us with 152 KB, 266 us with 76 KB). Small batches take more CTAs, to four per SM.
     const size_t share = (forward && grad ? 104u : 320u) << 10;
     uint32_t ctas = static_cast<uint32_t>(std::min<size_t>(kMaxCtas, (bytes + share - 1) / share));
     while (ctas < kMaxCtas && static_cast<size_t>(c.rows) * ctas < 4 * static_cast<size_t>(num_sms) &&
@@ -730,7 +822,7 @@ template <typename T>
 cudaError_t setup_typed() {
     // A bitmap of kDistillMaxVocab / kMaxCtas elements and the longest lists.
     const int most = static_cast<int>((kDistillMaxVocab / kMaxCtas / 32u + 3u) * sizeof(uint32_t) +
-                                      kDistillMaxTop * kEntryBytes + 16u);
+                                      kDistillMaxTop * kEntryBytes + 16u + kRingBytes);
     cudaError_t e = cudaFuncSetAttribute(distill_kernel<T, true, true>,
                                          cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e == cudaSuccess)
