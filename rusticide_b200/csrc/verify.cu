@@ -20,7 +20,10 @@
 //  1. verify_rows_kernel reads the rows of every test once (HBM-bound) and
 //     leaves a binary32 (reference, sum) per row part. (Ending a sequence's
 //     rows at a refusal seen meanwhile was tried: its flags and counters cost
-//     what it saved, 126 us against 123 at 96 x 7 x 128256.)
+//     what it saved, 126 us against 123 at 96 x 7 x 128256. So was one launch
+//     whose clusters sum their sequence's rows position by position and read
+//     none behind a refusal: 140 us against 119, and 40 against 27 at 8 x 5 x
+//     151936, since so few CTAs keep too few bytes in flight.)
 //  2. verify_draw_kernel, one cluster per sequence: decides the tests from
 //     those sums where their error bound allows it, sums the first undecided
 //     or refused position's rows once more in binary64, decides it exactly, and
@@ -113,8 +116,8 @@ __device__ __forceinline__ void visit_segment(const float *p, uint32_t lo, uint3
 
 // ---------------------------------------------------------------------------
 // Launch 1: a CTA per row part. Bound by HBM, with sixteen exponentials' worth
-// of loads in flight a thread: 96 x 7 x 128256 with ragged drafts reads 345 MB in
-// some 57 us (6 TB/s); the greedy form of 64 x 4 x 151936, 195 MB, in 38 us (5.1
+// of loads in flight a thread: 96 x 7 x 128256 with ragged drafts (383 of them)
+// reads 393 MB in 67 us under a profiler (5.8 TB/s); the greedy form of 64 x 4 x 151936, 195 MB, in 39 us (5.0
 // TB/s, the same with 2, 4 and 8 loads in flight and with 4 to 16 parts a row).
 // ---------------------------------------------------------------------------
 struct RowItem {
@@ -511,6 +514,10 @@ __device__ __forceinline__ double residual_weight(double sum_d, double sum_q, do
     return s;
 }
 
+// 96 x 7 x 128256: 65 us for the 72 MB of rows that it reads a second time. It is
+// bound by the latency of its chains of binary64 and table operations at two CTAs
+// an SM (issue slots 42 % busy, the binary64 pipe 21 %, DRAM 16 %); more threads,
+// CTAs or unrolling, with fewer registers each, took 116-125 us a call alike.
 __global__ void __launch_bounds__(kDrawThreads, 2)
 verify_draw_kernel(const __grid_constant__ VerifyCall c, uint32_t ctas) {
     extern __shared__ __align__(16) unsigned char draw_smem[];

@@ -293,6 +293,17 @@ def test_streams_and_graphs():
         assert torch.equal(grad, e.distill_backward(*a, state, up, tail=True))
 
 
+def test_replacing_logits_that_a_graph_keeps_is_noticed():
+    x, ids, y = case(3, 500, 8, seed=41)
+    x, a = x.cuda().requires_grad_(), (dev(ids), dev(y))
+    logits = x * 1.0
+    loss = distill_loss(logits, *a)
+    with torch.no_grad():
+        engine(0).distill_step(logits, *a, torch.ones(3, device="cuda"), out=logits)
+    with pytest.raises(RuntimeError, match="inplace operation"):
+        loss.sum().backward()
+
+
 def test_teacher_records_of_the_sampler():
     """The lists come from sample_ex as they are: survivors, their log-probabilities, their count."""
     rows, v = 6, 4001
