@@ -50,7 +50,7 @@ constexpr uint32_t kLoads = 4;    // 16-byte loads in flight per thread
 struct __align__(16) RowShare {
     float max_rest, sum_rest;      // over the tokens of the pass
     float max_listed, sum_listed;  // over the listed ones, with the tail
-    double cross, held;            // sums of t (y - y_ref - v) and of t over the CTA's entries
+    double cross, held;            // sums of t (y - y_ref - (v - v_ref)) and of t over the CTA's entries
 };
 
 struct DistillShared {
@@ -60,6 +60,7 @@ struct DistillShared {
     double red_t[kWarps];
     RowShare share[kMaxCtas];
     uint32_t unordered;
+    float v_ref;  // v of the row's first entry: what a loss is put together against
     float4 row;  // maximum, 1 / sum, unlisted maximum, unlisted factor
 };
 
@@ -97,14 +98,14 @@ __device__ __forceinline__ __half from_float<__half>(float x) { return __float2h
 // fl(ref log2 e), one packed multiply-add for two of them. The exponent is
 // rounded once and c carries 2^-24 of it, |v - ref| 2^-22 in all; what mc and c
 // make the reference off by is the same factor for the whole row, slip (log2,
-// binary64), and is taken out of sums and factors. Where ref log2 e leaves
-// binary32 (`wide`) the exponent is (v - ref) log2 e instead.
+// binary64), and is taken out of sums and factors. It grows with ref; beyond
+// 2^24 (`wide`) the exponent is (v - ref) log2 e instead.
 struct ExpRef {
     float ref, c, mc;
     bool wide;
     __device__ __forceinline__ ExpRef(const DistillCall &call, float ref_)
         : ref(ref_), c(call.exp2_scale), mc(ref_ * 1.44269504f) {
-        wide = !(fabsf(mc) < kPosInf) && fabsf(ref) < kPosInf;
+        wide = !(fabsf(mc) < 0x1p+24f) && fabsf(ref) < kPosInf;
     }
     // 2^-slip, which a sum or factor of these exponentials is to be multiplied by.
     __device__ __forceinline__ double correction(const DistillCall &call) const {
@@ -559,6 +560,12 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bi
     // may replace the logits).
     for (uint32_t k = threadIdx.x; k < n; k += kThreads)
         e.v[k] = here(e.id[k]) ? __fmul_rn(elem_to_float<T>(x[e.id[k]]), c.scale) : kNegInf;
+    if (kForward && threadIdx.x == 32) {
+        uint32_t k = 0;
+        while (k < n && e.id[k] == kAbsent) ++k;
+        const float v = k < n ? __fmul_rn(elem_to_float<T>(x[e.id[k]]), c.scale) : 0.0f;
+        sh.v_ref = fabsf(v) < kPosInf ? v : 0.0f;
+    }
 
     Teacher te{};
     if (kForward && listed) {
@@ -622,7 +629,7 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bi
                 const double t = e.t[k];
                 if (!here(e.id[k]) || t == 0.0) continue;
                 cross += t * (static_cast<double>(e.y[k]) - static_cast<double>(te.y_ref) -
-                              static_cast<double>(e.v[k]));
+                              (static_cast<double>(e.v[k]) - static_cast<double>(sh.v_ref)));
                 held_t += t;
             }
             cross = warp_sum(cross);
@@ -765,13 +772,15 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bi
             const double held_all = warp_sum(lane < ctas ? sh.share[lane].held : 0.0);
             if (lane == 0) {
                 const float mr = sh.red_m[0], sr = sh.red_s[0];
-                const double lse = static_cast<double>(sh.row.x) + log(static_cast<double>(sh.red_s[1]));
-                loss += held_all * (c.tail ? lse : lse - log(te.sum));
-                if (te.r > 0.0) {
-                    loss += te.r * (log(te.r) + lse);
-                    loss -= te.r * (sr != 0.0f ? static_cast<double>(mr) + log(static_cast<double>(sr))
-                                               : static_cast<double>(kNegInf));
-                }
+                // log S against v_ref and against the unlisted maximum: as such it would
+                // lose log of the sum where the logits are large.
+                const double row_max = sh.row.x, log_sum = log(static_cast<double>(sh.red_s[1]));
+                loss += held_all * (row_max - static_cast<double>(sh.v_ref) + log_sum -
+                                    (c.tail ? 0.0 : log(te.sum)));
+                if (te.r > 0.0)
+                    loss += te.r * (sr != 0.0f ? log(te.r) + (row_max - static_cast<double>(mr)) + log_sum -
+                                                     log(static_cast<double>(sr))
+                                               : static_cast<double>(kPosInf));
                 c.loss[row] = te.some ? static_cast<float>(loss) : 0.0f;
             }
         }

@@ -45,13 +45,13 @@ def row(x, ids, y, temperature=1.0, tail=False):
         listed[ids] = True
         rest = np.zeros(len(x))
         if r > 0:
-            log_rest = -np.inf
+            log_rest = -np.inf  # against m: as such it would swallow the sums' logs where m is large
             if (~listed).any() and v[~listed].max() != -np.inf:
                 mr = v[~listed].max()
                 er = np.exp(v[~listed] - mr)
                 rest[~listed] = er / er.sum()
-                log_rest = mr + np.log(er.sum())
-            loss = loss + r * (np.log(r) - log_rest + m + np.log(total))
+                log_rest = (mr - m) + np.log(er.sum())
+            loss = loss + r * (np.log(r) - log_rest + np.log(total))
         dense = np.zeros(len(x))
         np.add.at(dense, ids, t)
         grad = p * mass - r * rest - dense

@@ -174,6 +174,83 @@ def test_masked_logits_nan_and_infinities(tail):
     check(x, ids, y, tail=tail, up=up)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tail", [False, True])
+def test_masks_nan_and_infinities_in_long_rows(dtype, tail):
+    """Segments of several batches of 16-byte words, on their way through shared memory."""
+    v = 131077 * (1 if dtype is torch.float32 else 2)
+    x, ids, y = case(12, v, 8, seed=23, dtype=dtype)
+    g = torch.Generator().manual_seed(24)
+    x[torch.rand(x.shape, generator=g) < 0.3] = float("-inf")
+    for r in range(12):
+        x[r, ids[r].astype(np.int64)] = 0.5
+    x[0, int(ids[0, 2])] = float("-inf")
+    x[1] = float("-inf")
+    x[2, v // 2] = float("nan")
+    x[3, v - 1] = float("inf")
+    x[4] = float("-inf")
+    x[4, ids[4].astype(np.int64)] = 1.0
+    x[5] = torch.finfo(dtype).min
+    x[5, ids[5].astype(np.int64)] = 0.0
+    x[6, v // 3:] = float("-inf")             # whole segments without a logit
+    x[6, ids[6].astype(np.int64)] = 0.5
+    y[7, :] = -np.inf
+    n = np.full(12, 8, np.int32)
+    n[8], n[9] = 0, 3
+    up = np.linspace(0.5, 1.5, 12).astype(np.float32)
+    up[2], up[10] = 0.0, 0.0
+    check(x, ids, y, n=n, tail=tail, up=up)
+
+
+@pytest.mark.parametrize("v", [700, 131077])
+@pytest.mark.parametrize("tail", [False, True])
+def test_logits_next_to_the_largest_number(v, tail):
+    """Logits whose product with log2(e) leaves binary32; their neighbours are 2e31 away."""
+    x, ids, y = case(4, v, 8, seed=25)
+    for r, top in enumerate((3e38, 2.5e38, -3e38, 1e30)):
+        x[r] = -3.3e38
+        x[r, ::3] = top
+        x[r, ids[r].astype(np.int64)] = top
+    check(x, ids, y, tail=tail)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_strides_and_alignment_of_long_rows(dtype):
+    rows, v = 3, 131077 * (1 if dtype is torch.float32 else 2)
+    x, ids, y = case(rows, v, 12, seed=52, dtype=dtype)
+    up = np.ones(rows, np.float32)
+    want = R.batch(x.float().numpy(), ids, y, None, 1.0, True)
+    e = engine(0)
+    for offset in (0, 1, 4, 7):
+        buf = torch.full((rows * (v + 21) + 16,), float("nan"), dtype=dtype, device="cuda")
+        view = torch.as_strided(buf, (rows, v), (v + 21, 1), offset)
+        view.copy_(x)
+        loss, grad = e.distill_step(view, dev(ids), dev(y), dev(up), tail=True)
+        close_loss(loss, want[0])
+        close_grad(grad, want, up, 1.0, True)
+        e.distill_step(view, dev(ids), dev(y), dev(up), tail=True, out=view)
+        assert torch.equal(view, grad)
+        gap = torch.ones_like(buf, dtype=torch.bool)
+        torch.as_strided(gap, (rows, v), (v + 21, 1), offset).fill_(False)
+        assert buf[gap].isnan().all()
+
+
+def test_rows_far_apart():
+    """Row offsets that pass 32 bits, in elements and in bytes."""
+    rows, v, pitch = 3, 5003, 1200000007
+    x, ids, y = case(rows, v, 12, seed=53, dtype=torch.bfloat16)
+    up = np.ones(rows, np.float32)
+    want = R.batch(x.float().numpy(), ids, y, None, 1.0, False)
+    buf = torch.empty(2 * pitch + v, dtype=torch.bfloat16, device="cuda")
+    view = torch.as_strided(buf, (rows, v), (pitch, 1))
+    view.copy_(x)
+    loss, grad = engine(0).distill_step(view, dev(ids), dev(y), dev(up))
+    close_loss(loss, want[0])
+    close_grad(grad, want, up, 1.0, False)
+    engine(0).distill_step(view, dev(ids), dev(y), dev(up), out=view)
+    assert torch.equal(view, grad)
+
+
 def test_nearly_all_mass_on_the_listed_tokens():
     """The unlisted share is 1e-9 to 1e-13: it is summed as such, not as 1 minus the rest."""
     x, ids, y = case(4, 3000, 10, seed=31, spread=1.0, held=1 - 1e-6)

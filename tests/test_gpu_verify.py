@@ -173,6 +173,23 @@ def test_strides_and_alignment(offset):
         same([o.cpu().numpy() for o in out], want)
 
 
+def test_rows_far_apart():
+    """Offsets of sequences and rows that pass 32 bits, in elements and in bytes."""
+    b, d, v, far = 2, 1, 5003, 2300000004
+    x, y, t, u = case(b, d, v, seed=33)
+    want = R.verify_batch(x, y, t, None, u, 1.0)
+    buf = torch.empty(far + far // 2 + 3 * v, device="cuda")
+    target = torch.as_strided(buf, (b, d + 1, v), (far, far // 2, 1), 0)
+    draft = torch.as_strided(buf, (b, d, v), (far, v, 1), v)
+    target.copy_(torch.from_numpy(x))
+    draft.copy_(torch.from_numpy(y))
+    out = engine(0).verify(target, dev(t), FULL, uniforms=dev(u), draft_logits=draft)
+    same([o.cpu().numpy() for o in out], want)
+    greedy = SamplingParams(0.0, 0, 1.0)
+    out = engine(0).verify(target, dev(t), greedy)
+    same([o.cpu().numpy() for o in out], R.greedy_batch(x, t, None))
+
+
 @pytest.mark.parametrize("v", [1, 5, 4099, 151936])
 def test_greedy(v):
     b, d = 9, 5
