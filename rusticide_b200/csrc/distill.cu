@@ -22,11 +22,12 @@
 // summed over the unlisted tokens as such (a bitmap of the listed ones masks
 // them out): S minus the listed terms would lose it where the listed tokens
 // hold nearly all of the mass. Measured (B200, GPU time): loss of 4096 x 128256
-// bf16 with 128 entries and the tail 187 us (5.6 TB/s), loss and gradient of 2048
-// x 151936 bf16 231 us (5.4 TB/s of one read and one write). Keeping the segment
+// bf16 with 128 entries and the tail 190 us (5.5 TB/s), loss and gradient of 2048
+// x 151936 bf16 234 us (5.3 TB/s of one read and one write). Keeping the segment
 // in shared memory between the passes (TMA copies, four CTAs of 52 KB an SM)
 // took 305-322 us: the phases of so few CTAs do not overlap.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include <cooperative_groups.h>
@@ -94,24 +95,26 @@ template <>
 __device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
 
 // Exponentials of a row against a reference value `ref` (any number near its
-// largest v): exp(v - ref) = 2^(x c - mc) * 2^-slip with c = fl(s log2 e) and mc =
-// fl(ref log2 e), one packed multiply-add for two of them. The exponent is
-// rounded once and c carries 2^-24 of it, |v - ref| 2^-22 in all; what mc and c
-// make the reference off by is the same factor for the whole row, slip (log2,
-// binary64), and is taken out of sums and factors. It grows with ref; beyond
-// 2^24 (`wide`) the exponent is (v - ref) log2 e instead.
+// largest v): exp(v - ref) = 2^(v c - mc) * 2^-slip with c = fl(log2 e) and mc =
+// fl(ref c), one packed multiply-add for two of them. v = x s is rounded as the
+// listed tokens' is; where s is a power of two that product is exact and goes into
+// c (kExact: 2048 x 151936 bf16 234-240 us, with the product 241). The exponent is
+// rounded once (2^-24) and c is 1.3e-8 off, |v - ref| 2^-23 in all; exponentials
+// below 2^-126 are 0. What mc makes the reference off by is the same factor for the
+// whole row, slip (log2, binary64), and is taken out of sums and factors. It grows
+// with ref; beyond 2^24 (`wide`) the exponent is (v - ref) log2 e instead.
+constexpr float kLog2e = 1.44269504f;
 struct ExpRef {
-    float ref, c, mc;
+    float ref, mc;
     bool wide;
-    __device__ __forceinline__ ExpRef(const DistillCall &call, float ref_)
-        : ref(ref_), c(call.exp2_scale), mc(ref_ * 1.44269504f) {
+    __device__ __forceinline__ explicit ExpRef(float ref_) : ref(ref_), mc(ref_ * kLog2e) {
         wide = !(fabsf(mc) < 0x1p+24f) && fabsf(ref) < kPosInf;
     }
     // 2^-slip, which a sum or factor of these exponentials is to be multiplied by.
-    __device__ __forceinline__ double correction(const DistillCall &call) const {
+    __device__ __forceinline__ double correction() const {
         if (wide) return 1.0;
-        const double z = -0.6931471805599453 *
-                         __fma_rn(static_cast<double>(ref), call.exp2_ratio, -static_cast<double>(mc));
+        const double z = -0.6931471805599453 * __fma_rn(static_cast<double>(ref), static_cast<double>(kLog2e),
+                                                        -static_cast<double>(mc));
         // |z| is 1e-7 of |ref|; its cube / 6 is below 2e-13 in the short form.
         return fabs(z) < 1e-4 ? __fma_rn(z, __fma_rn(z, 0.5, 1.0), 1.0) : exp(z);
     }
@@ -161,13 +164,20 @@ __device__ __forceinline__ uint64_t mul_pair(uint64_t a, uint64_t b) {
     return d;
 }
 // Two neighbouring exponentials.
-__device__ __forceinline__ uint64_t exp_pair(uint64_t x, uint64_t c, uint64_t minus_mc) {
-    const uint64_t t = fma_pair(x, c, minus_mc);
+template <bool kExact>
+__device__ __forceinline__ uint64_t exp_pair(float x0, float x1, float scale, float mc) {
+    uint64_t v = pair_of(x0, x1);
+    float c = kLog2e;
+    if (kExact)
+        c = __fmul_rn(c, scale);
+    else
+        v = mul_pair(v, pair_of(scale, scale));
+    const uint64_t t = fma_pair(v, pair_of(c, c), pair_of(-mc, -mc));
     return pair_of(ex2_fast(low_of(t)), ex2_fast(high_of(t)));
 }
 __device__ __forceinline__ float exp_one(float x, float scale, const ExpRef &r) {
-    return r.wide ? exp_fast(__fsub_rn(__fmul_rn(x, scale), r.ref))
-                  : ex2_fast(__fmaf_rn(x, r.c, -r.mc));
+    const float v = __fmul_rn(x, scale);
+    return r.wide ? exp_fast(__fsub_rn(v, r.ref)) : ex2_fast(__fmaf_rn(v, kLog2e, -r.mc));
 }
 
 // The largest element of a 16-byte word (NaN passed over).
@@ -192,7 +202,7 @@ __device__ __forceinline__ float word_max<__half>(const uint4 &w) {
 }
 
 // A 16-byte word of the gradient from one of the logits: exp(v - ref) * factor.
-template <typename T, bool kWide>
+template <typename T, bool kWide, bool kExact>
 __device__ __forceinline__ uint4 grad_word(const uint4 &w, float scale, const ExpRef &r, float factor) {
     constexpr int kE = kVecElems<T>;
     float v[kE];
@@ -207,8 +217,7 @@ __device__ __forceinline__ uint4 grad_word(const uint4 &w, float scale, const Ex
             o.elem[i] = from_float<T>(__fmul_rn(exp_one(v[i], scale, r), factor));
             o.elem[i + 1] = from_float<T>(__fmul_rn(exp_one(v[i + 1], scale, r), factor));
         } else {
-            const uint64_t g = mul_pair(exp_pair(pair_of(v[i], v[i + 1]), pair_of(r.c, r.c), pair_of(-r.mc, -r.mc)),
-                                        pair_of(factor, factor));
+            const uint64_t g = mul_pair(exp_pair<kExact>(v[i], v[i + 1], scale, r.mc), pair_of(factor, factor));
             o.elem[i] = from_float<T>(low_of(g));
             o.elem[i + 1] = from_float<T>(high_of(g));
         }
@@ -378,8 +387,8 @@ struct Segment {
 };
 
 // The exponentials of kN 16-byte words added up as a tree.
-template <typename T, int kN>
-__device__ __forceinline__ float batch_sum(const uint4 *w, uint64_t c, uint64_t minus_mc) {
+template <typename T, int kN, bool kExact>
+__device__ __forceinline__ float batch_sum(const uint4 *w, float scale, float mc) {
     constexpr int kE = kVecElems<T>, kPairs = kN * kE / 2;
     uint64_t e[kPairs];
 #pragma unroll
@@ -387,7 +396,7 @@ __device__ __forceinline__ float batch_sum(const uint4 *w, uint64_t c, uint64_t 
         float v[kE];
         unpack<T>(w[k], v);
 #pragma unroll
-        for (int i = 0; i < kE; i += 2) e[(k * kE + i) / 2] = exp_pair(pair_of(v[i], v[i + 1]), c, minus_mc);
+        for (int i = 0; i < kE; i += 2) e[(k * kE + i) / 2] = exp_pair<kExact>(v[i], v[i + 1], scale, mc);
     }
 #pragma unroll
     for (int d = 1; d < kPairs; d *= 2) {
@@ -439,8 +448,8 @@ __device__ __forceinline__ void sum_segment(const DistillCall &c, const T *x, co
     // m stays -inf until there is a logit above it; the exponents' reference is
     // then 0, against which -inf gives 0 and NaN gives NaN.
     if (one > kNegInf) m = __fmul_rn(one, c.scale);
-    ExpRef r(c, m > kNegInf ? m : 0.0f);
-    double correction = r.correction(c);
+    ExpRef r(m > kNegInf ? m : 0.0f);
+    double correction = r.correction();
     s = static_cast<double>(exp_one(one, c.scale, r)) * correction;
     const uint4 *words = reinterpret_cast<const uint4 *>(x + seg.body);
     // A batch of words, the listed elements among them taken out.
@@ -471,8 +480,8 @@ __device__ __forceinline__ void sum_segment(const DistillCall &c, const T *x, co
             // Before the first logit above -inf the sum is 0 or NaN.
             if (m > kNegInf) s *= static_cast<double>(exp_fast(__fsub_rn(m, next)));
             m = next;
-            r = ExpRef(c, next);
-            correction = r.correction(c);
+            r = ExpRef(next);
+            correction = r.correction();
         }
         if (r.wide) {
             for (int k = 0; k < kN; ++k) {
@@ -481,7 +490,9 @@ __device__ __forceinline__ void sum_segment(const DistillCall &c, const T *x, co
                 for (uint32_t i = 0; i < kE; ++i) s += static_cast<double>(exp_one(v[i], c.scale, r));
             }
         } else {
-            s += static_cast<double>(batch_sum<T, kN>(w, pair_of(r.c, r.c), pair_of(-r.mc, -r.mc))) * correction;
+            const float sum = c.exact ? batch_sum<T, kN, true>(w, c.scale, r.mc)
+                                      : batch_sum<T, kN, false>(w, c.scale, r.mc);
+            s += static_cast<double>(sum) * correction;
         }
     };
     auto listed = [&](uint32_t q) -> uint32_t {
@@ -670,7 +681,7 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bi
                 factor = __fmul_rn(__fmul_rn(static_cast<float>(te.mass), exp_fast(__fsub_rn(mr, row_max))), inv);
                 if (te.r > 0.0) factor = __fsub_rn(factor, __fdiv_rn(static_cast<float>(te.r), sr));
             }
-            factor = __fmul_rn(factor, static_cast<float>(ExpRef(c, rest_max).correction(c)));
+            factor = __fmul_rn(factor, static_cast<float>(ExpRef(rest_max).correction()));
             if (!(all == all)) factor = all;
             if (lane == 0) {
                 sh.row = make_float4(row_max, inv, rest_max, factor);
@@ -703,7 +714,7 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bi
         // gradient, whatever its logits hold.
         const bool none = inv == 0.0f || up == 0.0f;
         const float by = __fmul_rn(up, c.scale);
-        const ExpRef r(c, rest_max);
+        const ExpRef r(rest_max);
         const float factor = __fmul_rn(by, rest_factor);
         auto one = [&](uint32_t j) {
             g[j] = from_float<T>(
@@ -719,34 +730,44 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bi
                 for (uint32_t q = threadIdx.x; q < seg.n_vec; q += kThreads) out[q] = make_uint4(0, 0, 0, 0);
             } else if (r.wide) {
                 for (uint32_t q = threadIdx.x; q < seg.n_vec; q += kThreads)
-                    out[q] = grad_word<T, true>(words[q], c.scale, r, factor);
+                    out[q] = grad_word<T, true, false>(words[q], c.scale, r, factor);
             } else {
-                uint32_t q0 = threadIdx.x;
-                if (kForward) {
-                    // From the segment's end, whose last batches are still there.
+                // One loop for each form of the exponent.
+                auto loop = [&](auto exact) {
+                    auto word = [&](const uint4 &w) {
+                        return grad_word<T, false, decltype(exact)::value>(w, c.scale, r, factor);
+                    };
+                    uint32_t q0 = threadIdx.x;
+                    if (kForward) {
+                        // From the segment's end, whose last batches are still there.
 #pragma unroll 1
-                    for (uint32_t b = ring.full; b-- > 0;) {
-                        uint4 w[kBatch];
-                        Ring::wait();
-                        ring.take(b, w);
-                        if (b >= kDepth) ring.fetch(b - kDepth);
-                        Ring::commit();
+                        for (uint32_t b = ring.full; b-- > 0;) {
+                            uint4 w[kBatch];
+                            Ring::wait();
+                            ring.take(b, w);
+                            if (b >= kDepth) ring.fetch(b - kDepth);
+                            Ring::commit();
 #pragma unroll
-                        for (uint32_t k = 0; k < kBatch; ++k)
-                            __stcs(out + q0 + (b * kBatch + k) * kThreads, grad_word<T, false>(w[k], c.scale, r, factor));
+                            for (uint32_t k = 0; k < kBatch; ++k)
+                                __stcs(out + q0 + (b * kBatch + k) * kThreads, word(w[k]));
+                        }
+                        q0 += ring.full * kThreads * kBatch;
                     }
-                    q0 += ring.full * kThreads * kBatch;
-                }
-                for (; !kForward && q0 + kThreads * (kLoads - 1) < seg.n_vec; q0 += kThreads * kLoads) {
-                    uint4 w[kLoads];
+                    for (; !kForward && q0 + kThreads * (kLoads - 1) < seg.n_vec; q0 += kThreads * kLoads) {
+                        uint4 w[kLoads];
 #pragma unroll
-                    for (uint32_t k = 0; k < kLoads; ++k) w[k] = __ldcs(words + q0 + k * kThreads);
+                        for (uint32_t k = 0; k < kLoads; ++k) w[k] = __ldcs(words + q0 + k * kThreads);
 #pragma unroll
-                    for (uint32_t k = 0; k < kLoads; ++k)
-                        __stcs(out + q0 + k * kThreads, grad_word<T, false>(w[k], c.scale, r, factor));
-                }
-                for (; q0 < seg.n_vec; q0 += kThreads)
-                    out[q0] = grad_word<T, false>(words[q0], c.scale, r, factor);
+                        for (uint32_t k = 0; k < kLoads; ++k)
+                            __stcs(out + q0 + k * kThreads, word(w[k]));
+                    }
+                    for (; q0 < seg.n_vec; q0 += kThreads)
+                        out[q0] = word(words[q0]);
+                };
+                if (c.exact)
+                    loop(std::true_type());
+                else
+                    loop(std::false_type());
             }
         } else {
             // The gradient's rows start at another 16-byte phase than the logits'.
@@ -852,8 +873,8 @@ cudaError_t distill_setup() {
 cudaError_t launch_distill(const DistillCall &call, rsc_dtype dtype, bool forward, bool grad, int num_sms,
                            cudaStream_t stream) {
     DistillCall c = call;
-    c.exp2_scale = c.scale * 1.44269504f;
-    c.exp2_ratio = static_cast<double>(c.exp2_scale) / static_cast<double>(c.scale);
+    int exponent = 0;
+    c.exact = std::frexp(c.scale, &exponent) == 0.5f;  // a power of two
     switch (dtype) {
         case RSC_F32: return launch_typed<float>(c, forward, grad, num_sms, stream);
         case RSC_BF16: return launch_typed<__nv_bfloat16>(c, forward, grad, num_sms, stream);

@@ -255,8 +255,7 @@ struct DistillCall {
     uint32_t rows, vocab;
     float scale;
     int tail;
-    float exp2_scale;   // scale * log2(e), and their quotient (set by launch_distill)
-    double exp2_ratio;
+    bool exact;             // scale is a power of two (set by launch_distill)
     const void *logits;
     size_t row_stride;
     size_t cap;             // teacher slots per row, at most kDistillMaxTop

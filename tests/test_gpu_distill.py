@@ -3,9 +3,10 @@
 Tolerances, from the arithmetic (rsc_rowsum.cuh): a sum of exponentials is within 6e-6 relative, so a
 log of it within 6e-6, and the loss, which holds at most two of them with weights that add up to
 1 + r <= 2, within 1.2e-5, plus a binary32 rounding of t (2^-24 relative of terms that add up to less
-than 40 here) and of the result. A gradient's p has |v - m| 2^-22 + 2^-22 from its exponential
-(|v - m| < 25 here where p is a normal number of the result: 6.2e-6), 6e-6 from the sum and four
-roundings (2.4e-7): 1.3e-5 relative, and so has the tail's r exp(v) / S_tail. The result is rounded to its type by at most half a step, relative eps / 2
+than 40 here) and of the result. A gradient's p has |v - m| 7.3e-8 + 2^-22 from its exponential
+(|v - m| < 88 where p is a normal number: 6.7e-6), 6e-6 from the sum and four roundings (2.4e-7):
+1.3e-5 relative, and so has the tail's r exp(v) / S_tail. Exponentials below 2^-126 are flushed to 0,
+and both sums are at least 1 against the largest term: 2^-126 of either, times the row's factor. The result is rounded to its type by at most half a step, relative eps / 2
 or half the smallest subnormal."""
 
 import numpy as np
@@ -58,7 +59,7 @@ def close_grad(got, want, up, temperature, tail):
     s = np.abs(up[:, None] * float(R.inverse(temperature)))
     rel = 1.3e-5 * size + 2e-7 * t
     tiny = float(info.smallest_normal * info.eps)
-    limit = s * rel + np.abs(value) * info.eps / 2 * 1.001 + max(tiny, 1e-37)
+    limit = s * (rel + 2 * 2.0 ** -126) + np.abs(value) * info.eps / 2 * 1.001 + max(tiny, 1e-37)
     assert np.array_equal(np.isnan(g), np.isnan(value))
     ok = np.isfinite(value)
     bad = np.abs(g[ok] - value[ok]) > limit[ok]
@@ -212,6 +213,24 @@ def test_logits_next_to_the_largest_number(v, tail):
         x[r, ::3] = top
         x[r, ids[r].astype(np.int64)] = top
     check(x, ids, y, tail=tail)
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("base", [3e4, 1e6, 1.1e7, 1.2e7, 3e7, 1e9, -1e6, -2e7])
+def test_logits_far_from_zero(base, tail):
+    """A common offset, on both sides of 2^24 / log2(e); the logits are what binary32 leaves of them."""
+    x, ids, y = case(6, 3001, 8, seed=26, spread=4.0)
+    check(x + base, ids, y, tail=tail, temperature=1.0)
+    check(x + base, ids, y, tail=tail, temperature=2.0)
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("temperature", [1e-4, 0.03, 0.3, 1.5, 70.0, 1e6, 1e30])
+@pytest.mark.parametrize("base", [0.0, 1000.0, -1e6])
+def test_temperatures(temperature, base, tail):
+    """v = x / T is rounded once, for listed and unlisted tokens alike."""
+    x, ids, y = case(6, 3001, 8, seed=27)
+    check(x + base, ids, y, tail=tail, temperature=temperature)
 
 
 @pytest.mark.parametrize("dtype", TYPES)

@@ -173,6 +173,15 @@ def test_strides_and_alignment(offset):
         same([o.cpu().numpy() for o in out], want)
 
 
+@pytest.mark.parametrize("base", [3e4, 1e6, 3e7, 1e9, -2e7, 1e30])
+def test_logits_far_from_zero(base):
+    """A common offset of all logits, which binary32 rounds to ever coarser steps."""
+    x, y, t, u = case(4, 3, 3001, seed=34, spread=4.0)
+    x, y = (x + np.float32(base)).astype(np.float32), (y + np.float32(base)).astype(np.float32)
+    same(run(x, y, t, u), R.verify_batch(x, y, t, None, u, 1.0))
+    same(run(x, None, t, u), R.verify_batch(x, None, t, None, u, 1.0))
+
+
 def test_rows_far_apart():
     """Offsets of sequences and rows that pass 32 bits, in elements and in bytes."""
     b, d, v, far = 2, 1, 5003, 2300000004
