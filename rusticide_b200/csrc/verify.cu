@@ -90,8 +90,8 @@ __device__ __forceinline__ float masked_scaled(float x, float scale) {
     return __fmul_rn(fmaxf(x, kNegInf), scale);  // fmaxf(NaN, -inf) = -inf; scale > 0
 }
 
-// Calls f(index, logit) for this thread's share of p[lo, hi): 16-byte loads
-// between the alignment head and tail, kLoads of them in flight.
+// Calls f(index, logit) for this thread's share of p[lo, hi) in ascending order:
+// 16-byte loads between the alignment head and tail, kLoads of them in flight.
 template <int kThreads, int kLoads, typename BatchF, typename OneF>
 __device__ __forceinline__ void visit_segment(const float *p, uint32_t lo, uint32_t hi, BatchF batch,
                                               OneF one) {
@@ -99,9 +99,9 @@ __device__ __forceinline__ void visit_segment(const float *p, uint32_t lo, uint3
     const uint32_t body = lo + min(hi - lo, (4u - mis) & 3u);
     const uint32_t n4 = (hi - body) / 4u;
     const uint32_t tail = body + 4u * n4;
+    const bool in_tail = threadIdx.x >= 32 && threadIdx.x - 32 < hi - tail;
+    const float last = in_tail ? p[tail + threadIdx.x - 32] : kNegInf;
     if (threadIdx.x < body - lo) one(lo + threadIdx.x, p[lo + threadIdx.x]);
-    if (threadIdx.x >= 32 && threadIdx.x - 32 < hi - tail)
-        one(tail + threadIdx.x - 32, p[tail + threadIdx.x - 32]);
     const float4 *p4 = reinterpret_cast<const float4 *>(p + body);
     for (uint32_t q0 = threadIdx.x; q0 < n4; q0 += kThreads * kLoads) {
         float4 x[kLoads];
@@ -112,6 +112,7 @@ __device__ __forceinline__ void visit_segment(const float *p, uint32_t lo, uint3
         }
         batch(body, q0, x);
     }
+    if (in_tail) one(tail + threadIdx.x - 32, last);
 }
 
 // ---------------------------------------------------------------------------
@@ -210,6 +211,7 @@ verify_greedy_rows_kernel(const __grid_constant__ VerifyCall c) {
     unsigned long long best = 0;
     uint32_t best_key = 0, finite = 0;
     auto visit = [&](uint32_t j, float x) {
+        // A thread's elements come in ascending order: the last of equal ones stays.
         const uint32_t key = total_key(masked_scaled(x, c.scale));
         if (key >= best_key) best_key = key, best = pack_key_index(key, j);
         finite |= fabsf(x) < kPosInf ? 1u : 0u;

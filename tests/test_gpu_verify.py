@@ -226,6 +226,38 @@ def test_greedy(v):
             assert want[0][i, want[1][i]] == ids[i, want[1][i]]
 
 
+@pytest.mark.parametrize("v", [1, 3, 4, 1027, 4096, 4097, 4098, 4099, 50001, 151936])
+@pytest.mark.parametrize("offset", [0, 1, 2, 3])
+def test_greedy_takes_the_last_of_equal_maxima(v, offset):
+    """Rows of one, two and three values, at every phase of their 16-byte words: the maximum stands
+    in the head, the body and the tail of each part, and the last of them counts."""
+    b, d = 6, 2
+    rng = np.random.default_rng(v + offset)
+    x = rng.integers(0, 3, size=(b, d + 1, v)).astype(np.float32)
+    x[0] = 1.0                                  # all equal
+    x[1] = np.minimum(x[1], 1.0)
+    x[2] = np.where(x[2] == 2.0, np.float32(0.0), np.float32(-0.0))  # total_cmp: -0 is below +0
+    x[3] = -np.inf
+    x[3, :, ::2] = -4.5                         # the even tokens are left, all equal
+    x[4] = np.finfo(np.float32).max             # +inf above finite logits, several times
+    x[4, :, :: max(1, v // 5)] = np.inf
+    x[4, :, 0] = 0.0
+    pitch = v + 5 + offset
+    buf = torch.zeros(b * (d + 1) * pitch + 8, device="cuda")
+    view = torch.as_strided(buf, x.shape, ((d + 1) * pitch, pitch, 1), offset)
+    view.copy_(torch.from_numpy(x))
+    flat = torch.as_strided(buf, (b * (d + 1), v), (pitch, 1), offset)
+    best = engine(0).greedy(flat)[0].cpu().numpy().reshape(b, d + 1)
+    t = best[:, :d].copy()                      # drafts that have to stand
+    t[5, 1] = (t[5, 1] + 1) % v if v > 1 else 1
+    want = R.greedy_batch(x, t, None)
+    for i in range(b):
+        assert want[0][i, want[1][i]] == best[i, want[1][i]] and want[2][i] == 0
+    assert (want[1][:5] == d).all()
+    out = engine(0).verify(view, dev(t), SamplingParams(0.0))
+    same([o.cpu().numpy() for o in out], want)
+
+
 def test_top_k_of_one_is_greedy():
     b, d, v = 4, 3, 999
     x, y, t, u = case(b, d, v, seed=41)
