@@ -304,24 +304,28 @@ verify_greedy_kernel(const __grid_constant__ VerifyCall c) {
 // ---------------------------------------------------------------------------
 
 // What exp(v - max) of a row is taken with; `max` is a reference that v exceeds
-// by 600 at most. Scaled logits more than 700 below it (-inf and NaN among them)
-// are raised to that floor, so that no term needs a branch; weights up to
-// kNoWeight, of terms 460 or more below it, count as 0 where a draw asks for the
-// first of any weight. Beyond 2^33
-// neighbouring binary32 numbers are 1024 apart: such a row is scaled down to
-// where they are 512 apart and the floor is next to the maximum, which leaves
-// every other token without weight, as it is.
+// by 500 at most. Scaled logits more than 512 below it (-inf and NaN among them)
+// are raised to that floor, so that no term needs a branch and none leaves the
+// normal numbers; weights up to kNoWeight, of terms 460 or more below it, the
+// floor's (4e-223) among them, count as 0 where a draw asks for the first of any
+// weight. max - 512 is a binary32 number as long as those below max are 512 apart
+// at most, up to 2^33. Beyond, every other token of the row is 512 or more below
+// its largest, out of reach of binary64's weights as it is: such a row is scaled
+// down by the power of two that leaves exactly 512 between the largest and what
+// is next below it, the floor. (Below a power of two itself numbers are half as
+// far apart as above it.)
 struct RowBase {
     float scale, max32, floor;
     double max;
     __device__ __forceinline__ RowBase() {}
     __device__ __forceinline__ RowBase(float scale_, float max_) : scale(scale_), max32(max_) {
         if (fabsf(max_) >= 0x1p+33f) {
-            const float down = scalbnf(1.0f, 32 - ilogbf(max_));
+            const int at = ilogbf(max_ > 0.0f ? nextafterf(max_, 0.0f) : max_);
+            const float down = scalbnf(1.0f, 32 - at);
             scale *= down;
             max32 *= down;
         }
-        floor = max32 - 700.0f;
+        floor = max32 - 512.0f;
         max = max32;
     }
 };
@@ -665,7 +669,8 @@ verify_draw_kernel(const __grid_constant__ VerifyCall c, uint32_t ctas) {
         if (!refused) {
             // The row behind the last test, of which nothing is known yet: each
             // warp sums against the maximum of its first block; binary64 holds
-            // terms up to 600 above that, a run with larger ones is summed again.
+            // terms up to 500 above that, a run with larger ones is summed again (as
+            // is any beyond 2^33, whose maximum RowBase has to know).
             float ref = kNegInf, top = kNegInf;
             double s = 0.0;
             while (true) {
@@ -682,7 +687,7 @@ verify_draw_kernel(const __grid_constant__ VerifyCall c, uint32_t ctas) {
                     for (int k = 0; k < kRowLoads; ++k) s += exp64(x[k], base, sh.tab);
                 });
                 top = warp_max(top);
-                if (top == ref || !(top < kPosInf) || static_cast<double>(top) - ref <= 600.0) break;
+                if (top == ref || !(top < kPosInf) || static_cast<double>(top) - ref <= 500.0) break;
                 ref = top;
                 s = 0.0;
             }

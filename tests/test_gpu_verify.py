@@ -182,6 +182,76 @@ def test_logits_far_from_zero(base):
     same(run(x, None, t, u), R.verify_batch(x, None, t, None, u, 1.0))
 
 
+def far_case(top, v, seed, below):
+    """Rows whose largest logit is `top`; the others are binary32 numbers below it, a step of
+    `below` apart and more, and a third of them masked. Drafts are the draft's likeliest token, a
+    masked one or, in two sequences, a token at the target's maximum."""
+    b, d = 8, 2
+    rng = np.random.default_rng(seed)
+    top = np.float32(top)
+
+    def rows(n):
+        gap = np.abs(rng.normal(size=(b, n, v))) * below + below
+        x = np.minimum(top - gap.astype(np.float32), np.nextafter(top, np.float32(-np.inf)))
+        x = x.astype(np.float32)
+        x[rng.random(x.shape) < 1 / 3] = -np.inf
+        at = rng.integers(0, v, size=(b, n, 3))     # the maximum, three times
+        np.put_along_axis(x, at, top, 2)
+        return x, at
+
+    x, at_x = rows(d + 1)
+    y, at_y = rows(d)
+    y[4:6, 0] = x[4:6, 0]                           # equal rows: accepted
+    at_y[4:6, 0] = at_x[4:6, 0]
+    t = at_y[:, :, 0].astype(np.int32)
+    t[6] = at_x[6, :d, 1]
+    masked = np.isneginf(x[2:4, 0])                 # of no probability, whatever the test draws
+    t[2:4, 0] = masked.argmax(1)
+    y[2, 0, t[2, 0]] = -np.inf                      # nor in the draft
+    u = rng.random((b, d + 1), dtype=np.float32) * np.float32(0.98) + np.float32(0.01)
+    u[7, :d] = np.float32(2.0 ** -24)
+    return x, y, t, u
+
+
+@pytest.mark.parametrize("v", [777, 40003])
+@pytest.mark.parametrize("top", [2.0 ** 29, 2.0 ** 30, 1.7e9, 2.0 ** 31, 2.2e9, 3e9, 4.2e9, 2.0 ** 32,
+                                 5e9, 8e9, 2.0 ** 33, 1e10, 2.0 ** 40, 1e20, 3.4e38, -1.7e9,
+                                 -2.0 ** 31, -3e9, -2.0 ** 32, -5e9, -2.0 ** 33, -1e10, -2.0 ** 40])
+def test_maxima_whose_neighbours_are_far_apart(top, v):
+    """Binary32 numbers are 64 apart and more here. Tokens a step below the maximum, masked ones and
+    the padding behind a row have no weight beside it, and none is drawn or accepted."""
+    x, y, t, u = far_case(top, v, seed=35, below=abs(top) * 2e-7)
+    for q in (y, None):
+        want = R.verify_batch(x, q, t, None, u, 1.0)
+        assert len(set(want[1])) > 1
+        same(run(x, q, t, u), want)
+
+
+@pytest.mark.parametrize("temperature", [1e-9, 1e-8, 1e-6, 1e-4, 1e-3])
+@pytest.mark.parametrize("top", [2.2, 4.0, 10.0, 25.0, 42.9, -3.0])
+def test_temperatures_near_zero(temperature, top):
+    """Almost greedy sampling of ordinary logits."""
+    for v in (1, 3001):
+        x, y, t, u = far_case(top, v, seed=36, below=0.25)
+        for q in (y, None):
+            same(run(x, q, t, u, SamplingParams(temperature, 0, 1.0)),
+                 R.verify_batch(x, q, t, None, u, temperature))
+
+
+@pytest.mark.parametrize("low,high", [(-2.0 ** 33, -2.0 ** 33 + 512), (2.0 ** 33 - 512, 2.0 ** 33),
+                                      (2.0 ** 33, 2.0 ** 33 + 1024), (2.0 ** 32 - 256, 2.0 ** 32)])
+def test_equal_maxima_met_early_and_late(low, high):
+    """Two tokens share the maximum; a warp meets one of them behind its first block of a row of
+    neighbouring numbers, another warp in its first block. Each has half of p."""
+    v = 151936
+    x = np.full((4, 1, v), low, np.float32)
+    x[:2, 0, [700, 2433]] = high
+    x[2:, 0, [1, 150000]] = high
+    u = np.array([[0.25], [0.75], [0.25], [0.75]], np.float32)
+    got = run(x, None, np.zeros((4, 0), np.int32), u)
+    assert got[0][:, 0].tolist() == [700, 2433, 1, 150000] and not got[2].any()
+
+
 def test_rows_far_apart():
     """Offsets of sequences and rows that pass 32 bits, in elements and in bytes."""
     b, d, v, far = 2, 1, 5003, 2300000004
