@@ -485,8 +485,10 @@ typedef struct rsc_draft_batch {
  * top-k off (0 or >= vocab) and top_p >= 1 (RSC_ERR_INVALID_ARGUMENT
  * otherwise: such a distribution is verified from its records, below) and a
  * finite 1/T > 0. Parameters of the argmax branch (T == 0 or top_k == 1)
- * verify greedily: t_i is accepted iff it is the token rsc_greedy gives for
- * the row, the last token is that of row a, and the draft rows are not read.
+ * verify greedily: t_i is accepted iff it is the token rsc_pick gives for the
+ * row with these parameters (T == 0: rsc_greedy's; top_k == 1: rsc_sample's, which
+ * compares scaled logits), the last token is that of row a, a row for which that
+ * call has RSC_ROW_NO_VALID_TOKENS has it here, and the draft rows are not read.
  *
  * d_workspace: rsc_verify_workspace_bytes(n_seqs, max_drafts, vocab) bytes, 16-byte
  * aligned, not initialised, free again when the call's work on the stream is

@@ -819,6 +819,7 @@ rsc_status rsc_verify(rsc_sampler *s, const rsc_draft_batch *x, const rsc_params
     rsc::VerifyCall c = verify_call(*x, d_uniforms, d_rng_states, d_out_tokens, d_out_accepted, d_out_status);
     c.vocab = static_cast<uint32_t>(x->vocab);
     c.scale = cp.scale;
+    c.finite_max = params->temperature != 0.0f;
     c.target = x->d_target;
     c.target_seq_stride = x->target_seq_stride;
     c.target_row_stride = x->target_row_stride;

@@ -221,6 +221,7 @@ struct VerifyRecords {
 struct VerifyCall {
     uint32_t n_seqs, max_drafts, vocab;
     float scale;
+    bool finite_max;      // greedy: a row's largest scaled logit has to be finite (not just any logit)
     const float *target;  // row i of sequence b at target + b * target_seq_stride + i * target_row_stride
     size_t target_seq_stride, target_row_stride;
     const float *draft;   // nullable

@@ -264,7 +264,10 @@ verify_greedy_rows_kernel(const __grid_constant__ VerifyCall c) {
 
 // ---------------------------------------------------------------------------
 // Greedy verification, launch 2: one warp per sequence. It reads a few words a
-// row and is bound by their latency.
+// row and is bound by their latency. What a row answers, and whether it answers, is
+// as rsc_pick has it: T = 0 goes by the logits and wants one finite among them, as
+// rsc_greedy does; top_k = 1 at another T goes by the scaled logits, as rsc_sample
+// does, whose softmax has no value where the largest of them is infinite.
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(128)
 verify_greedy_kernel(const __grid_constant__ VerifyCall c) {
@@ -283,7 +286,8 @@ verify_greedy_kernel(const __grid_constant__ VerifyCall c) {
         const uint32_t finite =
             __reduce_or_sync(0xffffffffu, lane < c.parts ? parts[lane].any_finite : 0u);
         best = warp_max(best);
-        if (!finite) {
+        const uint32_t key = static_cast<uint32_t>(best >> 32);
+        if (c.finite_max ? key <= kKeyNegInf || key >= kKeyPosInf : !finite) {
             status = RSC_ROW_NO_VALID_TOKENS;
             break;
         }

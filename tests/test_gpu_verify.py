@@ -335,6 +335,45 @@ def test_top_k_of_one_is_greedy():
     same(run(x, y, t, u, SamplingParams(0.7, 1, 0.9)), R.greedy_batch(x, t, None))
 
 
+@pytest.mark.parametrize("temperature", [0.0, 0.7, 1.0, 3.0, 1e-30, -1.0])
+def test_greedy_parameters_give_the_sampler_s_tokens(temperature):
+    """The argmax branch of the sampler: T = 0 compares the logits themselves, top_k = 1 the scaled
+    ones, where neighbouring logits can become equal and the last of them counts. What rsc_pick
+    answers for a row is what its draft is compared with."""
+    v, d = 1003, 1
+    rng = np.random.default_rng(43)
+    x = rng.normal(size=(300, d + 1, v)).astype(np.float32)
+    high = (5 + 15 * rng.random(300)).astype(np.float32)
+    at = np.sort(rng.choice(v, size=(300, 2)), axis=1)
+    for i in range(200):                        # the two largest are neighbours, the larger one first
+        x[i, :, at[i, 0]], x[i, :, at[i, 1]] = np.nextafter(high[i], np.float32(99)), high[i]
+    x[200, 0, 5] = np.inf
+    x[201] = -np.inf
+    x[202, 0] = np.nan
+    x[203, 0, ::2] = -np.inf
+    x[204, 0] = 1e-45                           # equal after a product that underflows
+    x[204, 0, 7] = 3e-45
+    x[205, 0] = -np.inf
+    x[205, 0, 3] = np.inf
+    x[206] = 3e38
+    params = SamplingParams(temperature, 1, 1.0)
+    rows = dev(x).reshape(-1, v)
+    ids, status, _ = engine(0).pick(rows, params, uniforms=torch.zeros(len(rows), device="cuda"))
+    ids, status = ids.cpu().numpy().reshape(300, 2), status.cpu().numpy().reshape(300, 2) & 0xFF
+    t = np.where(status[:, :1] == 0, ids[:, :1], 0).astype(np.int32)
+    out = engine(0).verify(dev(x), dev(t), params)
+    tokens, accepted, st = [o.cpu().numpy() for o in out]
+    for i in range(300):
+        a = 0 if status[i, 0] else 1
+        assert accepted[i] == a and st[i] == status[i, a]
+        want = [-1, -1]
+        if a:
+            want[0] = ids[i, 0]
+        if not st[i]:
+            want[a] = ids[i, a]
+        assert tokens[i].tolist() == want
+
+
 def test_generator_states():
     """Draws from per-sequence states equal the same draws given as uniforms, and a state advances
     by what its sequence consumed."""
