@@ -310,14 +310,16 @@ verify_greedy_kernel(const __grid_constant__ VerifyCall c) {
 // What exp(v - max) of a row is taken with; `max` is a reference that v exceeds
 // by 500 at most. Scaled logits more than 512 below it (-inf and NaN among them)
 // are raised to that floor, so that no term needs a branch and none leaves the
-// normal numbers; weights up to kNoWeight, of terms 460 or more below it, the
-// floor's (4e-223) among them, count as 0 where a draw asks for the first of any
-// weight. max - 512 is a binary32 number as long as those below max are 512 apart
-// at most, up to 2^33. Beyond, every other token of the row is 512 or more below
-// its largest, out of reach of binary64's weights as it is: such a row is scaled
-// down by the power of two that leaves exactly 512 between the largest and what
-// is next below it, the floor. (Below a power of two itself numbers are half as
-// far apart as above it.)
+// normal numbers. A token whose weight is kNoWeight of the largest or less, 460 or
+// more below it, the floor's 4e-223 among them, is none that a test accepts or a
+// draw takes; up to 2^31 of them add up to kNoSum at most.
+//
+// max - 512 is a binary32 number as long as those below max are 512 apart at
+// most, up to 2^33. Beyond, every other token of the row is 512 or more below its
+// largest, out of reach of binary64's weights as it is: such a row is scaled down
+// by the power of two that leaves exactly 512 between the largest and what is
+// next below it, the floor. (Below a power of two itself numbers are half as far
+// apart as above it.)
 struct RowBase {
     float scale, max32, floor;
     double max;
@@ -334,6 +336,7 @@ struct RowBase {
     }
 };
 constexpr double kNoWeight = 1e-200;
+constexpr double kNoSum = 1e-190;
 
 constexpr uint32_t kExpSteps = 512;  // entries of the table 2^(j / kExpSteps)
 
@@ -426,6 +429,9 @@ struct DrawShared {
     // What each warp's position was tested with: u, and both rows' logits of the token.
     float test_u[kDrawWarps], test_p[kDrawWarps], test_q[kDrawWarps];
     uint32_t test_token[kDrawWarps];
+    // Weights up to this are none: of CTAs on the row's scale, of tokens on the CTA's.
+    double none_row, none;
+    float bonus_max;  // the largest scaled logit of the row behind the last test, when that is drawn from
 };
 
 // [lo, hi) cut into kDrawWarps runs whose length is a multiple of 32.
@@ -500,8 +506,8 @@ __device__ __forceinline__ double warp_scan(double s) {
 // Of the lanes' sums of weights, the first whose running total exceeds `rest`;
 // `rest` becomes what is wanted within it. Where rounding leaves none, the last
 // lane of any weight, with all of it wanted. The same in every lane.
-__device__ __forceinline__ uint32_t locate(double s, double &rest) {
-    const bool some = s > kNoWeight;
+__device__ __forceinline__ uint32_t locate(double s, double none, double &rest) {
+    const bool some = s > none;
     const double upto = warp_scan(s);
     const uint32_t hit = __ballot_sync(0xffffffffu, some && upto > rest);
     const uint32_t any = __ballot_sync(0xffffffffu, some);
@@ -524,6 +530,34 @@ __device__ __forceinline__ double residual_weight(double sum_d, double sum_q, do
     return s;
 }
 
+// The first token of weight at `hi` or behind it, else the last one before `lo`; the
+// whole block, apart from the draw (whose registers it would cost).
+__device__ __noinline__ uint32_t nearest_token(Draw d, uint32_t lo, uint32_t hi, uint32_t vocab, DrawShared &sh) {
+    auto counts = [&](uint32_t j) {
+        return j < vocab &&
+               weight_of(d, j, d.p[j], d.weight == kWeightResidual ? d.q[j] : 0.0f, sh.tab) > kNoWeight;
+    };
+    if (threadIdx.x == 0) sh.first = vocab;
+    bool any = false;
+    for (uint32_t k = hi; !any && k < vocab; k += kDrawThreads) {
+        const bool hit = counts(k + threadIdx.x);
+        any = __syncthreads_or(hit);
+        if (hit) atomicMin(&sh.first, k + threadIdx.x);
+    }
+    if (!any) {
+        __syncthreads();
+        if (threadIdx.x == 0) sh.first = 0;
+        for (uint32_t k = (lo + kDrawThreads - 1) / kDrawThreads; !any && k-- > 0;) {
+            const uint32_t j = k * kDrawThreads + threadIdx.x;
+            const bool hit = j < lo && counts(j);
+            any = __syncthreads_or(hit);
+            if (hit) atomicMax(&sh.first, j);
+        }
+    }
+    __syncthreads();
+    return sh.first;
+}
+
 // 96 x 7 x 128256: 65 us for the 72 MB of rows that it reads a second time. It is
 // bound by the latency of its chains of binary64 and table operations at two CTAs
 // an SM (issue slots 42 % busy, the binary64 pipe 21 %, DRAM 16 %); more threads,
@@ -538,6 +572,10 @@ verify_draw_kernel(const __grid_constant__ VerifyCall c, uint32_t ctas) {
     const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
     for (uint32_t j = threadIdx.x; j < kExpSteps; j += kDrawThreads)
         sh.tab[j] = exp2(static_cast<double>(j) / kExpSteps);
+    if (threadIdx.x == 0) {
+        sh.none_row = sh.none = kNoWeight;
+        sh.bonus_max = kNegInf;
+    }
     const uint32_t n = drafts_of(c, b);
     const uint32_t *drafts = c.draft_tokens + static_cast<size_t>(b) * c.max_drafts;
     const uint32_t seg = ((c.vocab + ctas - 1) / ctas + 31u) & ~31u;
@@ -718,6 +756,13 @@ verify_draw_kernel(const __grid_constant__ VerifyCall c, uint32_t ctas) {
             cta_weight = cta_sum(0) * (lane < ctas ? exp(refs - row_ref) : 0.0);
             d.base_p = RowBase(c.scale, cta_ref);
             own_scale = exp(row_ref - static_cast<double>(cta_ref));
+            // References may lie below the row's maximum, which has the say on weights.
+            if (threadIdx.x == 0) {
+                sh.bonus_max = static_cast<float>(row_top);
+                const double none_row = kNoWeight * exp(row_top - row_ref);
+                sh.none_row = none_row;
+                sh.none = none_row * own_scale;
+            }
             if (threadIdx.x < kDrawWarps) sh.warp_weight[threadIdx.x] = sh.warp_sum[threadIdx.x][0];
             total = warp_sum(cta_weight);
             break;
@@ -833,7 +878,7 @@ verify_draw_kernel(const __grid_constant__ VerifyCall c, uint32_t ctas) {
             }
             total = warp_sum(cta_weight);
         }
-        if (!(total > kNoWeight)) {
+        if (!(total > kNoSum)) {
             // Nothing is left (p and q are equal, the token was outside both): p itself.
             d.weight = kWeightRow;
             share(run_sum(d, wlo, whi, sh.tab), 0.0, 0.0, 0.0, 0u);
@@ -843,7 +888,7 @@ verify_draw_kernel(const __grid_constant__ VerifyCall c, uint32_t ctas) {
         }
         break;
     }
-    __syncthreads();  // warp_weight is complete
+    __syncthreads();  // warp_weight and none are complete
 
     uint32_t *out = c.out_tokens + static_cast<size_t>(b) * (c.max_drafts + 1);
     if (rank == 0) {
@@ -862,11 +907,11 @@ verify_draw_kernel(const __grid_constant__ VerifyCall c, uint32_t ctas) {
     if (status == RSC_ROW_OK) {
         constexpr uint32_t kTail = 8;
         double rest = static_cast<double>(c.uniforms ? last_u : uniform_of(c, b, tests, true)) * total;
-        if (locate(cta_weight, rest) == rank) {
+        if (locate(cta_weight, sh.none_row, rest) == rank) {
             rest *= own_scale;
             uint32_t flo = lo, fhi = hi;
             while (true) {
-                const uint32_t w = locate(lane < kDrawWarps ? sh.warp_weight[lane] : 0.0, rest);
+                const uint32_t w = locate(lane < kDrawWarps ? sh.warp_weight[lane] : 0.0, sh.none, rest);
                 uint32_t nlo, nhi;
                 warp_run(flo, fhi, w, nlo, nhi);
                 flo = nlo;
@@ -887,27 +932,36 @@ verify_draw_kernel(const __grid_constant__ VerifyCall c, uint32_t ctas) {
                 w[k] = 0.0;
                 if (k < each && j < fhi) {
                     w[k] = weight_of(d, j, d.p[j], d.weight == kWeightResidual ? d.q[j] : 0.0f, sh.tab);
-                    if (!(w[k] > kNoWeight)) w[k] = 0.0;
+                    if (!(w[k] > sh.none)) w[k] = 0.0;
                 }
                 sum += w[k];
             }
             const double upto = warp_scan(sum);
-            __syncthreads();
-            if (lane == 31) sh.warp_weight[warp] = upto;
-            __syncthreads();
-            if (locate(lane < kDrawWarps ? sh.warp_weight[lane] : 0.0, rest) == warp &&
-                locate(sum, rest) == lane) {
-                double run = 0.0;
-                uint32_t token = j0;
-                bool found = false;
+            if (__syncthreads_or(sum > 0.0)) {
+                if (lane == 31) sh.warp_weight[warp] = upto;
+                __syncthreads();
+                if (locate(lane < kDrawWarps ? sh.warp_weight[lane] : 0.0, 0.0, rest) == warp &&
+                    locate(sum, 0.0, rest) == lane) {
+                    double run = 0.0;
+                    uint32_t token = j0;
+                    bool found = false;
 #pragma unroll
-                for (uint32_t k = 0; k < kTail; ++k) {
-                    if (found || w[k] == 0.0) continue;
-                    run += w[k];
-                    token = j0 + k;
-                    found = run > rest;
+                    for (uint32_t k = 0; k < kTail; ++k) {
+                        if (found || w[k] == 0.0) continue;
+                        run += w[k];
+                        token = j0 + k;
+                        found = run > rest;
+                    }
+                    out[a] = token;
                 }
-                out[a] = token;
+            } else {
+                // The run was found for the sum of tokens that are none by themselves: a
+                // draw of u = 0, or the sums' rounding at a row's end. The first
+                // token of weight behind it is meant, or the last one before it (one of
+                // them exists, the total being above kNoSum).
+                if (sh.bonus_max != kNegInf) d.base_p = RowBase(c.scale, sh.bonus_max);
+                const uint32_t token = nearest_token(d, flo, fhi, c.vocab, sh);
+                if (threadIdx.x == 0) out[a] = token;
             }
         }
     }

@@ -252,6 +252,43 @@ def test_equal_maxima_met_early_and_late(low, high):
     assert got[0][:, 0].tolist() == [700, 2433, 1, 150000] and not got[2].any()
 
 
+@pytest.mark.parametrize("v", [40003, 151936])
+@pytest.mark.parametrize("copies", [1, 40])
+def test_tokens_without_weight_are_not_drawn_for_their_number(v, copies):
+    """465 below the maximum a token has no probability, and neither have a hundred thousand of them.
+    A draw of u = 0 takes the first token of any probability, which is the last one here; masked
+    tokens stand in front."""
+    x = np.full((3, 2, v), -465.0, np.float32)
+    x[:, :, :5000] = -np.inf
+    x[:, :, v - 1] = 0.0
+    x[1:, 0, v // 2] = 0.0                      # sequences 1 and 2: half of p each, one refused
+    y = np.full((3, 1, v), -np.inf, np.float32)
+    y[:, 0, v // 2] = 0.0
+    t = np.full((3, 1), v // 2, np.int32)
+    u = np.array([[0.5, 0.0], [0.75, 0.0], [0.75, 0.0]], np.float32)
+    n = np.array([0, 1, 1], np.int32)
+    many = [np.concatenate([a] * copies) for a in (x, y, t, u, n)]
+    for q in (many[1], None):
+        tokens, accepted, status = run(many[0], q, *many[2:4], n=many[4])
+        assert not accepted.any() and not status.any()
+        assert (tokens[:, 0] == v - 1).all() and (tokens[:, 1] == -1).all()
+
+
+@pytest.mark.parametrize("copies", [1, 40])
+def test_what_counts_as_weight_is_measured_from_the_largest_logit(copies):
+    """480 below it a token has no probability, however early in the row and wherever the maximum
+    stands: a draw of u = 0 passes over it."""
+    v, places = 151936, [0, 600, 1500, 9000, 100100, 151935]
+    x = np.zeros((len(places), 1, v), np.float32)
+    for i, at in enumerate(places):
+        x[i, 0, at] = 480.0
+    x = np.concatenate([x] * copies)
+    u = np.zeros((len(x), 1), np.float32)
+    tokens, _, status = run(x, None, np.zeros((len(x), 0), np.int32), u)
+    assert not status.any()
+    assert tokens[:, 0].tolist() == places * copies
+
+
 def test_rows_far_apart():
     """Offsets of sequences and rows that pass 32 bits, in elements and in bytes."""
     b, d, v, far = 2, 1, 5003, 2300000004
