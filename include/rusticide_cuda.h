@@ -548,7 +548,9 @@ RSC_API rsc_status rsc_verify_survivors(rsc_sampler *sampler, const rsc_draft_ba
  * y is taken as given: for a temperature the teacher's rows are sampled at that
  * temperature (its log-probabilities are of the scaled logits). Entries with an
  * id outside the vocabulary (the padding of the lists) or y = -inf are absent;
- * an id listed twice counts twice in the loss and once in sum p. A row without
+ * an id listed twice counts twice in the loss and once in sum p. A list that
+ * rsc_sample_ex cut short (d_n above cap) counts as the entries it holds, the
+ * first ids of the survivors: give it slots for all of them. A row without
  * an entry has loss 0 and no gradient. A student logit of -inf has p = 0 (a
  * listed one gives loss +inf); a NaN or +inf logit, or a row of -inf alone,
  * gives NaN, as a log-softmax does.
@@ -569,7 +571,8 @@ typedef struct rsc_distill_batch {
     int tail;
     float temperature;        /* > 0, 1/T finite                                        */
     size_t cap;               /* teacher slots per row                                  */
-    const uint32_t *d_n;      /* rows: entries of each row (above cap reads as cap); NULL: cap */
+    const uint32_t *d_n;      /* rows: entries of each row; NULL: cap. Above cap reads as cap, */
+                              /*   2^31 and above (a negative count) as 0                   */
     const uint32_t *d_ids;    /* rows x cap                                             */
     const float *d_logprobs;  /* rows x cap                                             */
 } rsc_distill_batch;

@@ -552,7 +552,7 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bi
     e.t = e.y + c.cap;
     e.v = e.t + c.cap;
     uint32_t n = static_cast<uint32_t>(c.cap);
-    if (c.n) n = min(n, c.n[row]);
+    if (c.n) n = min(n, static_cast<uint32_t>(max(0, static_cast<int32_t>(c.n[row]))));
     // A row with an empty list is not looked at (for every CTA of the cluster alike).
     const bool listed = n > 0;
     float *state = c.state ? c.state + row * 4 : nullptr;

@@ -44,8 +44,10 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor
                  tail: bool = False) -> torch.Tensor:
     """Loss of every row of student logits [..., vocab] against a teacher's top tokens ids
     [..., top] int32 with log-probabilities logprobs [..., top] f32 (see rsc_distill in the C
-    header), n [...] int32 of them a row. Returns [...] f32; differentiable once, with respect to
-    the logits. A training loop that knows each row's weight beforehand takes
+    header), n [...] int32 of them a row (None: all; below 0: none). A count above `top` reads as
+    `top`, as the lists of a sample_ex call have it whose survivor_cap was too small for a row: they
+    hold the first ids of its survivors, not the likeliest, so give that call slots for all.
+    Returns [...] f32; differentiable once, with respect to the logits. A training loop that knows each row's weight beforehand takes
     `Engine.distill_step`, which gives loss and gradient in one pass."""
     if logits.requires_grad and torch.is_grad_enabled():
         return _DistillLoss.apply(logits, ids, logprobs, n, temperature, tail)

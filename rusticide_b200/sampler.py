@@ -581,8 +581,10 @@ class Engine:
                         tail: bool = False, want_state: bool = True):
         """rsc_distill without a gradient. Returns (loss [...] f32, state): the loss of every row of
         `logits` [..., vocab] (f32, bf16 or f16) against the teacher's entries ids [..., top] int32
-        and logprobs [..., top] f32, n [...] int32 of them (None: all; ids of -1 are skipped), and
-        the state that distill_backward takes (None without want_state)."""
+        and logprobs [..., top] f32, n [...] int32 of them (None: all; below 0: none; above `top`:
+        all; ids of -1 are skipped), and the state that distill_backward takes (None without
+        want_state). Lists that sample_ex cut short hold the first ids of the survivors, not the
+        likeliest: a count above `top` says so, and nothing here refuses it."""
         b, x = self._distill_batch(logits, ids, logprobs, n, temperature, tail)
         loss = logprobs.new_empty(logits.shape[:-1])
         state = logprobs.new_empty((b.rows, 4)) if want_state else None

@@ -140,6 +140,21 @@ def test_no_rows_and_no_entries(tail):
     check(x, ids, y, tail=tail)
 
 
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_a_negative_count_is_an_empty_list(dtype, tail):
+    x, ids, y = case(6, 3000, 8, seed=28, dtype=dtype)
+    n = np.array([-1, 8, -2 ** 31, 0, 9, 3], np.int32)
+    loss, grad = check(x, ids, y, n=n.clip(0), tail=tail)
+    e, a = engine(0), (dev(x), dev(ids), dev(y))
+    kw, up = dict(n=dev(n), tail=tail), dev(np.linspace(0.5, 2.0, 6).astype(np.float32))
+    got, state = e.distill_forward(*a, **kw)
+    assert torch.equal(got, loss) and not got[[0, 2, 3]].any()
+    both, step = e.distill_step(*a, up, **kw)
+    assert torch.equal(step, grad) and not step[[0, 2, 3]].any()
+    assert not e.distill_backward(*a, state, up, **kw)[[0, 2, 3]].any()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 @pytest.mark.parametrize("tail", [False, True])
 def test_lists_out_of_order_and_with_repeats(dtype, tail):
