@@ -12,6 +12,7 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from .sampler import Engine, engine
 
@@ -49,6 +50,9 @@ def distill_loss(logits: torch.Tensor, ids: torch.Tensor, logprobs: torch.Tensor
     hold the first ids of its survivors, not the likeliest, so give that call slots for all.
     Returns [...] f32; differentiable once, with respect to the logits. A training loop that knows each row's weight beforehand takes
     `Engine.distill_step`, which gives loss and gradient in one pass."""
+    if (forward_ad.unpack_dual(logits).tangent is not None
+            or forward_ad.unpack_dual(logprobs).tangent is not None):
+        raise NotImplementedError("distill_loss has no forward-mode derivative")
     if logits.requires_grad and torch.is_grad_enabled():
         return _DistillLoss.apply(logits, ids, logprobs, n, temperature, tail)
     return _engine_of(logits).distill_forward(logits, ids, logprobs, n, temperature, tail,

@@ -124,3 +124,17 @@ def test_distill_loss_needs_a_gpu():
         pytest.skip("this machine has one")
     with pytest.raises(RuntimeError):
         distill_loss(**arguments())
+
+
+@pytest.mark.parametrize("name", ["logits", "logprobs"])
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(name, grad):
+    """A tangent must not be dropped: a dual tensor has no requires_grad of its own to go by."""
+    with torch.autograd.forward_ad.dual_level():
+        a = arguments()
+        a[name] = torch.autograd.forward_ad.make_dual(a[name].requires_grad_(grad), torch.ones_like(a[name]))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            distill_loss(**a)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="CUDA"):  # no tangent: the call goes on
+            distill_loss(**arguments())
