@@ -451,8 +451,9 @@ RSC_API rsc_status rsc_shard_collect(const uint32_t *d_ready_results, uint32_t s
  *     positive weight should rounding find none.
  * Every decision is that of exact arithmetic on the given binary32 values, to
  * 1e-13 relative. A token whose scaled logit is 465 or more below its row's
- * largest has no probability, one 460 below it may or may not (it takes a u of 0
- * to see it), and a rest p_a - q_a of less than 1e-190 in all is nothing left.
+ * largest has no probability, one 455 below it may or may not (it takes a u of 0,
+ * or a drafted token that its draft gives next to none, to see that), and a rest
+ * p_a - q_a of less than 1e-190 in all is nothing left.
  * But for such tokens results do not depend on the batch around a sequence.
  *
  * d_out_tokens[b] (max_drafts + 1 uint32): the accepted tokens, the drawn one,

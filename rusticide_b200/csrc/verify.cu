@@ -767,12 +767,19 @@ verify_draw_kernel(const __grid_constant__ VerifyCall c, uint32_t ctas) {
             total = warp_sum(cta_weight);
             break;
         }
-        const float max_p = sh.max_p[at], max_q = sh.max_q[at];
-        const double guess = sh.kappa[at];
+        float max_p = sh.max_p[at], max_q = sh.max_q[at];
+        double guess = sh.kappa[at];
         const bool paired = c.draft != nullptr;
         if (!(fabsf(max_p) < kPosInf) || (paired && !(fabsf(max_q) < kPosInf))) {
             status = RSC_ROW_NO_VALID_TOKENS;
             break;
+        }
+        // References near one another become one, so that equal logits have equal
+        // terms: rows that are the same leave nothing, although their alignment
+        // may have led to two references.
+        if (paired && max_p != max_q && fabsf(max_p - max_q) <= kHeadroom) {
+            guess *= exp(static_cast<double>(max_p) - static_cast<double>(max_q));
+            max_p = max_q = fmaxf(max_p, max_q);
         }
         d.base_p = RowBase(c.scale, max_p);
         d.base_q = RowBase(c.scale, max_q);

@@ -105,6 +105,21 @@ def test_equal_distributions_accept_every_token():
     assert (got[1] == d).all()
 
 
+@pytest.mark.parametrize("v", [6, 15, 42, 1003, 20001])
+def test_equal_rows_leave_nothing_whatever_their_alignment(v):
+    """A token outside the vocabulary is refused; where the draft's row is the target's, nothing is
+    left of it and the last token is drawn from the row itself."""
+    b, d = 24, 3
+    rng = np.random.default_rng(v)
+    for spread in (0.05, 0.7, 6.0):
+        x = (rng.normal(size=(b, d + 1, v)) * spread).astype(np.float32)
+        y = x[:, :d].copy()
+        t = rng.integers(0, v, size=(b, d)).astype(np.int32)
+        t[np.arange(b), rng.integers(0, d, size=b)] = [-1, v] * (b // 2)
+        u = rng.random((b, d + 1), dtype=np.float32)
+        same(run(x, y, t, u, SamplingParams(0.7, 0, 1.0)), R.verify_batch(x, y, t, None, u, 0.7))
+
+
 def test_edges_of_a_test():
     """u exactly at p / q refuses (the test is strict); one step below accepts."""
     v = 4
