@@ -450,11 +450,10 @@ RSC_API rsc_status rsc_shard_collect(const uint32_t *d_ready_results, uint32_t s
  *     running weight exceeds u * (sum of the weights), the last one of
  *     positive weight should rounding find none.
  * Every decision is that of exact arithmetic on the given binary32 values, to
- * 1e-13 relative. A token whose scaled logit is 465 or more below its row's
- * largest has no probability, one 455 below it may or may not (it takes a u of 0,
- * or a drafted token that its draft gives next to none, to see that), and a rest
- * p_a - q_a of less than 1e-190 in all is nothing left.
- * But for such tokens results do not depend on the batch around a sequence.
+ * 1e-13 relative, and results do not depend on the batch around a sequence. A
+ * token of 1e-200 or less of the likeliest one's probability, whose scaled logit is
+ * 461 or more below the row's largest, has none; a rest p_a - q_a of 1e-190 or
+ * less of it in all is nothing left.
  *
  * d_out_tokens[b] (max_drafts + 1 uint32): the accepted tokens, the drawn one,
  * then 0xffffffff. d_out_accepted[b] = a. d_out_status[b] is RSC_ROW_OK, or

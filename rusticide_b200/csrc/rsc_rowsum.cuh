@@ -5,12 +5,15 @@
 // a reference at most kHeadroom below the largest v. A thread takes its logits in
 // batches of 16: the batch's maximum first, then sixteen exponentials against one
 // reference, added as a tree in binary32 and once per batch into a binary64 sum.
+// At its end a thread brings the sum to its largest v itself, so that the reference
+// of a row is its maximum, however the row is cut.
 // Its error has three parts. An exponential is ex2.approx of a product rounded
-// once, |v - m| 2^-23 + 2^-22 relative. A new reference, and the join of lanes,
-// warps and parts, scales a sum by one more of them; references rise by more than
-// kHeadroom, so the terms that count, within 25 of the largest, see at most six,
-// and their distances add up to that 25: 3e-6 + 10 * 2^-22 in all. The trees are
-// four additions deep (2^-22). Together below 6e-6.
+// once, |v - m| 2^-23 + 2^-22 relative. A new reference, the thread's maximum, and
+// the join of lanes, warps and parts, scales a sum by one more of them; references
+// rise by more than kHeadroom, so the terms that count, within 25 of the largest,
+// see at most six, and their distances add up to that 25 and twice kHeadroom (a v
+// above m): 4e-6 + 11 * 2^-22 in all. The trees are four additions deep (2^-22).
+// Together below 7e-6 (6e-6 where the reference stays, as in distillation).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -75,14 +78,15 @@ __device__ __forceinline__ float exp_fast(float d) {
 
 constexpr float kHeadroom = 4.0f;
 
-// Adds kN scaled logits to (m, s). A logit of -inf adds nothing; +inf makes m
+// Adds kN scaled logits to (m, s) and raises `top` to their largest. A logit of -inf adds nothing; +inf makes m
 // +inf and s NaN, and NaN makes s NaN (callers that read NaN as -inf fold it
 // beforehand).
 template <int kN>
-__device__ __forceinline__ void sum_batch(float &m, double &s, const float *v) {
+__device__ __forceinline__ void sum_batch(float &m, float &top, double &s, const float *v) {
     float b = v[0];
 #pragma unroll
     for (int i = 1; i < kN; ++i) b = fmaxf(b, v[i]);
+    top = fmaxf(top, b);
     if (b > m + kHeadroom) {
         // m = -inf only while s is 0 or NaN, which the product keeps.
         s *= m == kNegInf ? 1.0 : static_cast<double>(exp_fast(__fsub_rn(m, b)));
@@ -100,6 +104,12 @@ __device__ __forceinline__ void sum_batch(float &m, double &s, const float *v) {
         for (int i = 0; i + w < kN; i += 2 * w) e[i] = __fadd_rn(e[i], e[i + w]);
     }
     s = __dadd_rn(s, static_cast<double>(e[0]));
+}
+
+// A thread's sum brought to its largest v.
+__device__ __forceinline__ void sum_to_top(float &m, float top, double &s) {
+    if (top > m) s *= static_cast<double>(exp_fast(__fsub_rn(m, top)));
+    m = top;
 }
 
 // The sums of `width` neighbouring lanes joined, in every one of them: the

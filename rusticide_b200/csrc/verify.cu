@@ -48,7 +48,7 @@ constexpr int kDrawWarps = kDrawThreads / 32;
 constexpr uint32_t kDrawMaxCtas = 16;  // the largest cluster (8 is the largest portable one)
 
 // Part of a row, as the first launch leaves it: (m, sum of exp(v - m)) with m
-// near the largest v (rsc_rowsum.cuh), or for greedy calls the packed
+// the largest v (rsc_rowsum.cuh), or for greedy calls the packed
 // (total-order key, index) of the largest logit and whether any logit is finite.
 struct RowPart {
     union {
@@ -162,7 +162,7 @@ verify_rows_kernel(const __grid_constant__ VerifyCall c) {
     part_bounds(c, r.part, lo, hi);
     const float *p = r.draft ? draft_row(c, r.b, r.i) : target_row(c, r.b, r.i);
 
-    float m = kNegInf;
+    float m = kNegInf, top = kNegInf;
     double s = 0.0;
     visit_segment<kRowThreads, 4>(
         p, lo, hi,
@@ -175,12 +175,13 @@ verify_rows_kernel(const __grid_constant__ VerifyCall c) {
                 v[4 * k + 2] = masked_scaled(x[k].z, c.scale);
                 v[4 * k + 3] = masked_scaled(x[k].w, c.scale);
             }
-            sum_batch<16>(m, s, v);
+            sum_batch<16>(m, top, s, v);
         },
         [&](uint32_t, float x) {
             const float v = masked_scaled(x, c.scale);
-            sum_batch<1>(m, s, &v);
+            sum_batch<1>(m, top, s, &v);
         });
+    sum_to_top(m, top, s);
     sum_join_lanes(m, s, 32);
     if ((threadIdx.x & 31) == 0) {
         red_m[threadIdx.x >> 5] = m;
@@ -307,11 +308,11 @@ verify_greedy_kernel(const __grid_constant__ VerifyCall c) {
 // Launch 2: decisions and the last token.
 // ---------------------------------------------------------------------------
 
-// What exp(v - max) of a row is taken with; `max` is a reference that v exceeds
-// by 500 at most. Scaled logits more than 512 below it (-inf and NaN among them)
+// What exp(v - max) of a row is taken with; `max` is its maximum, or a reference
+// that v exceeds by 500 at most. Scaled logits more than 512 below it (-inf and NaN among them)
 // are raised to that floor, so that no term needs a branch and none leaves the
-// normal numbers. A token whose weight is kNoWeight of the largest or less, 460 or
-// more below it, the floor's 4e-223 among them, is none that a test accepts or a
+// normal numbers. A token whose weight is kNoWeight of the largest or less, 460.5
+// or more below it, the floor's 4e-223 among them, is none that a test accepts or a
 // draw takes; up to 2^31 of them add up to kNoSum at most.
 //
 // max - 512 is a binary32 number as long as those below max are 512 apart at
@@ -685,7 +686,7 @@ verify_draw_kernel(const __grid_constant__ VerifyCall c, uint32_t ctas) {
                 if (valid && test_token < c.vocab) {
                     const double left = test_u * s * (c.draft ? eq : 1.0);
                     const double right = e * (c.draft ? sq : 1.0);
-                    // Each sum is within 6e-6 of its value.
+                    // Each sum is within 7e-6 of its value.
                     certain = left * (1.0 + 3e-5) < right;
                 }
                 if (!certain) atomicMin(&sh.first, i);
@@ -767,20 +768,15 @@ verify_draw_kernel(const __grid_constant__ VerifyCall c, uint32_t ctas) {
             total = warp_sum(cta_weight);
             break;
         }
-        float max_p = sh.max_p[at], max_q = sh.max_q[at];
-        double guess = sh.kappa[at];
+        const float max_p = sh.max_p[at], max_q = sh.max_q[at];
+        const double guess = sh.kappa[at];
         const bool paired = c.draft != nullptr;
         if (!(fabsf(max_p) < kPosInf) || (paired && !(fabsf(max_q) < kPosInf))) {
             status = RSC_ROW_NO_VALID_TOKENS;
             break;
         }
-        // References near one another become one, so that equal logits have equal
-        // terms: rows that are the same leave nothing, although their alignment
-        // may have led to two references.
-        if (paired && max_p != max_q && fabsf(max_p - max_q) <= kHeadroom) {
-            guess *= exp(static_cast<double>(max_p) - static_cast<double>(max_q));
-            max_p = max_q = fmaxf(max_p, max_q);
-        }
+        // The rows' own maxima: the same for rows that are the same, which leave
+        // nothing of one another, and a row's only likely token has a term of 1.
         d.base_p = RowBase(c.scale, max_p);
         d.base_q = RowBase(c.scale, max_q);
         const uint32_t t = sh.test_token[at];

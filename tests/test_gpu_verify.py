@@ -304,6 +304,41 @@ def test_what_counts_as_weight_is_measured_from_the_largest_logit(copies):
     assert tokens[:, 0].tolist() == places * copies
 
 
+@pytest.mark.parametrize("v", [1003, 151936])
+@pytest.mark.parametrize("copies", [1, 60])
+def test_where_weight_ends(v, copies):
+    """1e-200 of the largest, between 460 and 461 below it, in draws and tests of u = 0, wherever
+    the maximum stands and however a row is cut."""
+    for shift in (0.0, -1000.0, 77.25):
+        x = np.full((4, 2, v), -np.inf, np.float32)
+        for i, at in enumerate((v - 1, v // 2, v - 1, v // 3)):
+            x[i, :, v // 4:] = shift - 3.0      # in front of the maximum and behind it
+            x[i, :, at] = shift
+            x[i, :, 1] = shift - (460.0 if i < 2 else 461.0)
+        t = np.full((4, 1), 1, np.int32)
+        many = [np.concatenate([a] * copies) for a in (x, t, np.zeros((4, 2), np.float32))]
+        tokens, accepted, _ = run(many[0], None, *many[1:])
+        want = [[1, 1], [1, 1], [v // 4, -1], [v // 4, -1]]
+        assert tokens.tolist() == want * copies
+        assert accepted.tolist() == [1, 1, 0, 0] * copies
+
+
+def test_one_likely_token_in_both_rows():
+    """A token that has all of p and all of q, to binary64's last place, leaves the unlikely ones."""
+    b, v = 40, 3001
+    rng = np.random.default_rng(44)
+    x = (rng.normal(size=(b, 2, v)) * 2 - 60).astype(np.float32)
+    y = (x[:, :1] + rng.normal(size=(b, 1, v))).astype(np.float32)
+    at = rng.integers(0, v, size=b)
+    for i in range(b):
+        x[i, :, at[i]], y[i, 0, at[i]] = 10 * rng.random(), 10 * rng.random()
+    t = np.full((b, 1), v, np.int32)            # outside: refused
+    u = rng.random((b, 2), dtype=np.float32)
+    want = R.verify_batch(x, y, t, None, u, 1.0)
+    assert (want[0][:, 0] != at).any()
+    same(run(x, y, t, u), want)
+
+
 def test_rows_far_apart():
     """Offsets of sequences and rows that pass 32 bits, in elements and in bytes."""
     b, d, v, far = 2, 1, 5003, 2300000004
