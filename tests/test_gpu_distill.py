@@ -218,6 +218,24 @@ def test_masks_nan_and_infinities_in_long_rows(dtype, tail):
     check(x, ids, y, n=n, tail=tail, up=up)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tail", [False, True])
+def test_the_loss_is_the_same_with_and_without_the_state(dtype, tail):
+    """Bit for bit, in rows of NaN and infinite loss as in the others."""
+    x, ids, y = case(12, 40001, 8, seed=29, dtype=dtype)
+    x[1] = float("-inf")
+    x[2, 5] = float("nan")
+    x[3, 6] = float("inf")
+    x[4, int(ids[4, 1])] = float("-inf")
+    y[5, 1] = np.nan
+    e, a = engine(0), (dev(x), dev(ids), dev(y))
+    loss, state = e.distill_forward(*a, tail=tail)
+    alone, none = e.distill_forward(*a, tail=tail, want_state=False)
+    assert state is not None and none is None
+    assert torch.equal(loss.view(torch.int32), alone.view(torch.int32))
+    assert loss.isnan().tolist() == [r in (1, 2, 3, 5) for r in range(12)] and loss[4].isinf()
+
+
 @pytest.mark.parametrize("v", [700, 131077])
 @pytest.mark.parametrize("tail", [False, True])
 def test_logits_next_to_the_largest_number(v, tail):
