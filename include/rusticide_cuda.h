@@ -582,7 +582,8 @@ typedef struct rsc_distill_batch {
  * NULL, in the same launch the gradient d(sum_r row_grads[r] * loss[r]) /
  * d(logits) in the logits' type, rows grad_stride elements apart. A row with
  * row_grads[r] == 0 gets a gradient of 0. d_dlogits may be d_logits itself
- * (then grad_stride == row_stride): the gradient replaces the logits. d_state
+ * (then grad_stride == row_stride): the gradient replaces the logits; otherwise
+ * the two must not overlap. d_state
  * (rows x 4 f32, 16-byte aligned, nullable) keeps what rsc_distill_backward
  * needs of a row.
  *

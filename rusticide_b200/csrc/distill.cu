@@ -23,7 +23,8 @@
 // them out): S minus the listed terms would lose it where the listed tokens
 // hold nearly all of the mass. Measured (B200, GPU time): loss of 4096 x 128256
 // bf16 with 128 entries and the tail 190 us (5.5 TB/s), loss and gradient of 2048
-// x 151936 bf16 234 us (5.3 TB/s of one read and one write). Keeping the segment
+// x 151936 bf16 234 us (5.3 TB/s of one read and one write). Figures of variants
+// below are differences to these, each measured beside the kernel as it then was. Keeping the segment
 // in shared memory between the passes (TMA copies, four CTAs of 52 KB an SM)
 // took 305-322 us: the phases of so few CTAs do not overlap.
 #include <algorithm>
@@ -98,7 +99,7 @@ __device__ __forceinline__ __half from_float<__half>(float x) { return __float2h
 // largest v): exp(v - ref) = 2^(v c - mc) * 2^-slip with c = fl(log2 e) and mc =
 // fl(ref c), one packed multiply-add for two of them. v = x s is rounded as the
 // listed tokens' is; where s is a power of two that product is exact and goes into
-// c (kExact: 2048 x 151936 bf16 234-240 us, with the product 241). The exponent is
+// c (kExact, 2048 x 151936 bf16: up to 7 us less than with the product). The exponent is
 // rounded once (2^-24) and c is 1.3e-8 off, |v - ref| 2^-23 in all; exponentials
 // below 2^-126 are 0. What mc makes the reference off by is the same factor for the
 // whole row, slip (log2, binary64), and is taken out of sums and factors. It grows
@@ -328,9 +329,9 @@ __device__ __forceinline__ void join_lanes(float &m, float &s) {
 // asynchronously, so that the next ones travel while one is worked on. No other
 // thread reads them. The second pass goes from the segment's end, whose last
 // batches are still there. 48 KB a CTA leave four on an SM: 2048 x 151936 bf16
-// 233 us, against 258 with plain loads and six CTAs, 245 with six of 32 KB, 254 with
-// three of 64 KB, 240 with twelve words in batches of two. (The loss alone has no
-// second pass that stalls: six CTAs of plain loads, 188 us against 196 at 4096 x
+// takes 25 us more with plain loads and six CTAs, 12 with six of 32 KB, 21 with three
+// of 64 KB, 7 with twelve words in batches of two. (The loss alone has no second
+// pass that stalls: six CTAs of plain loads, 8 us less than the ring at 4096 x
 // 128256 bf16.)
 constexpr uint32_t kBatch = 4;
 constexpr uint32_t kDepth = 3;
@@ -770,7 +771,9 @@ distill_kernel(const __grid_constant__ DistillCall c, uint32_t ctas, uint32_t bi
                     loop(std::false_type());
             }
         } else {
-            // The gradient's rows start at another 16-byte phase than the logits'.
+            // The gradient's rows start at another 16-byte phase than the logits', as
+            // dense rows beside padded ones of an odd vocabulary: element by element
+            // (2048 x 151937 bf16 766 us, against 285 in place or with both dense).
             for (uint32_t j = lo + threadIdx.x; j < hi; j += kThreads) one(j);
         }
         // The listed tokens' gradients replace what the loop wrote there.
@@ -833,10 +836,12 @@ cudaError_t launch_typed(const DistillCall &c, bool forward, bool grad, int num_
     const size_t bytes = static_cast<size_t>(c.vocab) * sizeof(T);
     // A CTA's segment. The loss alone and the backward pass read a row once, and
     // every CTA of a row repeats the work on its list: whole rows up to 320 KB
-    // (2 x 160 KB costs 4096 x 128256 bf16 losses 231 us against 199). Loss and
+    // (2 x 160 KB costs 4096 x 128256 bf16 losses 32 us). Loss and
     // gradient together read the row twice, the second time from L2, which has to
     // hold what the CTAs of the GPU (four per SM) are at: 104 KB each (2048 x
-    // 151936 bf16: 233 us; 243 us with 152 KB, 266 us with 76 KB). Small batches take more CTAs, to four per SM.
+    // 151936 bf16 takes 10 us more with 152 KB, 33 with 76 KB). Small batches take
+    // more CTAs, to four per SM; a batch a little above one round of the GPU's CTAs
+    // (888 for the loss alone) pays for a second, nearly empty one.
     const size_t share = (forward && grad ? 104u : 320u) << 10;
     uint32_t ctas = static_cast<uint32_t>(std::min<size_t>(kMaxCtas, (bytes + share - 1) / share));
     while (ctas < kMaxCtas && static_cast<size_t>(c.rows) * ctas < 4 * static_cast<size_t>(num_sms) &&

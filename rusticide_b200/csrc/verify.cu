@@ -18,7 +18,7 @@
 //
 // Whole vocabulary, two launches:
 //  1. verify_rows_kernel reads the rows of every test once (HBM-bound) and
-//     leaves a binary32 (reference, sum) per row part. (Ending a sequence's
+//     leaves a binary32 (maximum, sum) per row part. (Ending a sequence's
 //     rows at a refusal seen meanwhile was tried: its flags and counters cost
 //     what it saved, 126 us against 123 at 96 x 7 x 128256. So was one launch
 //     whose clusters sum their sequence's rows position by position and read
@@ -118,7 +118,7 @@ __device__ __forceinline__ void visit_segment(const float *p, uint32_t lo, uint3
 // ---------------------------------------------------------------------------
 // Launch 1: a CTA per row part. Bound by HBM, with sixteen exponentials' worth
 // of loads in flight a thread: 96 x 7 x 128256 with ragged drafts (383 of them)
-// reads 393 MB in 67 us under a profiler (5.8 TB/s); the greedy form of 64 x 4 x 151936, 195 MB, in 39 us (5.0
+// reads 393 MB in 68 us under a profiler (5.8 TB/s); the greedy form of 64 x 4 x 151936, 195 MB, in 39 us (5.0
 // TB/s, the same with 2, 4 and 8 loads in flight and with 4 to 16 parts a row).
 // ---------------------------------------------------------------------------
 struct RowItem {
@@ -559,7 +559,7 @@ __device__ __noinline__ uint32_t nearest_token(Draw d, uint32_t lo, uint32_t hi,
     return sh.first;
 }
 
-// 96 x 7 x 128256: 65 us for the 72 MB of rows that it reads a second time. It is
+// 96 x 7 x 128256: 67 us for the 72 MB of rows that it reads a second time. It is
 // bound by the latency of its chains of binary64 and table operations at two CTAs
 // an SM (issue slots 42 % busy, the binary64 pipe 21 %, DRAM 16 %); more threads,
 // CTAs or unrolling, with fewer registers each, took 116-125 us a call alike.
@@ -980,8 +980,8 @@ verify_draw_kernel(const __grid_constant__ VerifyCall c, uint32_t ctas) {
 // Survivor records: one block per sequence, a warp per test, then one warp that
 // draws. The lists are short (top_k and its ties), so the call is bound by the
 // chain of dependent loads (token, list, bisection in the draft's list) and the
-// launch: one sequence of 4 drafts over 64 slots 5.5 us, 512 of 6 over 152 slots
-// 14.6 us.
+// launch: one sequence of 4 drafts over 64 slots 5.8 us, 512 of 6 over 152 slots
+// 14.9 us.
 // ---------------------------------------------------------------------------
 constexpr int kListThreads = 128;
 constexpr int kListWarps = kListThreads / 32;

@@ -598,8 +598,10 @@ class Engine:
                      out: Optional[torch.Tensor] = None):
         """rsc_distill with its gradient in the same pass: (loss [...], d(sum row_grads * loss) /
         d logits in the logits' type). row_grads [...] f32 is what each row's loss counts (its
-        weight over the batch size, 0 for padding). `out` takes the gradient; it may be `logits`
-        itself, which the gradient then replaces."""
+        weight over the batch size, 0 for padding). `out` takes the gradient, dense; it may be
+        `logits` itself, padded rows among them, which the gradient then replaces, and must not
+        overlap it otherwise. (Padded logits of an odd vocabulary are fastest in place: a dense
+        gradient's rows have another alignment.)"""
         b, x = self._distill_batch(logits, ids, logprobs, n, temperature, tail)
         up = self._want(row_grads, "row_grads", torch.float32, logits.shape[:-1])
         written = out is not None
